@@ -62,6 +62,24 @@ class Memory(C.Structure):
     _fields_ = [("weights", C.c_uint64), ("cache", C.c_uint64), ("scratch", C.c_uint64)]
 
 
+class Cache4(C.Structure):
+    _fields_ = [("k_quants", C.c_void_p), ("k_scales", C.c_void_p), ("v_quants", C.c_void_p), ("v_scales", C.c_void_p),
+                ("pages", C.c_uint32), ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32)]
+
+
+class Cache4Batch(C.Structure):
+    _fields_ = [("context", C.c_void_p), ("page_table", C.c_void_p), ("query_start", C.c_void_p), ("sequences", C.c_uint32),
+                ("table_columns", C.c_uint32), ("tokens", C.c_uint32), ("max_tokens", C.c_uint32), ("max_length", C.c_uint32)]
+
+
+class Cache4Rows(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_uint64),
+                ("k_stride", C.c_uint64), ("v_stride", C.c_uint64), ("q_out_stride", C.c_uint64), ("q_bias", C.c_void_p),
+                ("k_bias", C.c_void_p), ("v_bias", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+                ("rope_turns", C.c_void_p), ("rope_dim", C.c_uint32), ("rope_adjacent", C.c_int32), ("rope_attn_factor", C.c_float),
+                ("eps", C.c_float), ("heads", C.c_uint32), ("type", C.c_int32)]
+
+
 # Every symbol include/brisk_cuda.h declares, with its ctypes signature.
 SIGNATURES = {
     "brisk_cuda_device_count": (C.c_int, []),
@@ -83,6 +101,12 @@ SIGNATURES = {
     "brisk_cuda_matmul_seconds": (C.c_int, [C.c_int32, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32,
                                             C.c_uint32, C.POINTER(C.c_double), C.c_char_p, C.c_size_t]),
     "brisk_cuda_argmax_static": (C.c_int, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "brisk_cuda_rope_turns": (C.c_int, [C.c_uint32, C.c_double, C.c_double, _FP, C.POINTER(C.c_double), C.c_char_p, C.c_size_t]),
+    "brisk_cuda_cache4_append": (C.c_int, [C.POINTER(Cache4), C.POINTER(Cache4Batch), C.POINTER(Cache4Rows), C.c_void_p, C.c_char_p, C.c_size_t]),
+    "brisk_cuda_cache4_attention": (C.c_int, [C.POINTER(Cache4), C.POINTER(Cache4Batch), C.c_int32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64,
+                                              C.c_uint32, C.c_float, C.c_uint32, C.c_void_p, C.c_char_p, C.c_size_t]),
+    "brisk_cuda_cache4_read": (C.c_int, [C.POINTER(Cache4), C.POINTER(Cache4Batch), C.c_int32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64,
+                                         C.c_void_p, C.c_char_p, C.c_size_t]),
     "brisk_cuda_profile": (C.c_int, [C.c_void_p, C.c_int, C.c_char_p, C.c_size_t]),
     "brisk_cuda_debug_buffer": (C.c_int, [C.c_void_p, C.c_char_p, _FP, C.c_uint64]),
     "brisk_cuda_tp_unique_id": (C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t]),

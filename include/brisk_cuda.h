@@ -263,6 +263,90 @@ int brisk_cuda_matmul_seconds(int32_t type, const void* w, uint64_t rows, uint64
 int brisk_cuda_argmax_static(const float* logits, uint32_t vocab, uint32_t rows, int32_t* out_tokens, void* stream, char* err,
                              size_t errlen);
 
+/* ---- key/value cache in 4 bits, in pages ------------------------------------------------------------------------------
+ * No counterpart in the reference (its cache is f16, contiguous, of one sequence). For embedders that keep the keys and values of
+ * several sequences, or of long ones, in 28 % of the f16 bytes: rows are appended, attended to and read back by the three calls below.
+ * All pointers are DEVICE pointers on the current device unless
+ * they are said to be host ones; `stream` is a cudaStream_t (NULL: the default stream). The calls launch on the stream and return: no
+ * allocation, no synchronisation, no workspace, nothing kept - they may be captured into a graph and replayed, with context,
+ * page_table and query_start read at every replay. They return 0, or -1 and a message in err before anything is launched.
+ *
+ * A head's row of one position is head_dim / 32 blocks of 32 values: a scale d, and 16 bytes in the order of a Q4_0 block (byte j: value j
+ * in the low, value j + 16 in the high four bits); a value is (n - 8) d. Appending chooses d = -m / 8, m the block's value of largest
+ * magnitude (the positive one of two), rounded to 8 significant bits and kept as f16 (at most 65280), and n = floor(x / d + 8.5)
+ * within 0 .. 15 (8 where d is 0). With 8 significant bits a value is an f16 number exactly. A NaN is stored as 0, an infinity as
+ * the largest value of its block. */
+typedef struct brisk_cuda_cache4 {
+    void* k_quants; /* [pages][kv_heads][page_size][head_dim / 2] bytes; every plane starts on a 16-byte boundary */
+    void* k_scales; /* [pages][kv_heads][page_size][head_dim / 32] f16 */
+    void* v_quants;
+    void* v_scales;
+    uint32_t pages;
+    uint32_t page_size; /* positions of a page: 16 to 4096, a power of two */
+    uint32_t kv_heads;
+    uint32_t head_dim;  /* 64, 128 or 256 */
+} brisk_cuda_cache4;
+
+/* Tokens of several sequences one behind the other: token i of sequence s is row query_start[s] + i of q, k, v and the outputs and
+ * stands at position context[s] + i. Rows behind the last sequence's are not touched; a sequence may have no tokens, and no positions
+ * before them. A page number outside the pool is no error: its positions are not written and read as rows of zeros; so are positions
+ * past the table's columns, which attention does not see at all. Two columns of the sequences that append to one page, at the same
+ * position, leave either's row. */
+typedef struct brisk_cuda_cache4_batch {
+    const int32_t* context;     /* [sequences] positions before this batch's tokens                                        */
+    const int32_t* page_table;  /* [sequences][table_columns]; NULL: column c of sequence s is page s * table_columns + c   */
+    const int32_t* query_start; /* [sequences + 1], ascending; NULL: tokens / sequences each                               */
+    uint32_t sequences;
+    uint32_t table_columns;
+    uint32_t tokens;     /* rows of q, k, v and the outputs                                                                 */
+    uint32_t max_tokens; /* no sequence has more tokens in this batch; 0: tokens. Ignored where query_start is NULL. Attention does
+                            not compute a sequence's tokens past it                                                          */
+    uint32_t max_length; /* no sequence has more positions, these tokens included; 0: what the columns hold. How the work is split
+                            goes by it; results are right whatever it says                                                   */
+} brisk_cuda_cache4_batch;
+
+/* One layer's projections of a batch: element (row, head, i) of q is at q[row * q_stride + head * head_dim + i], the others likewise
+ * (strides in values; q, k and v may lie in one fused buffer, and q_out may be q). */
+typedef struct brisk_cuda_cache4_rows {
+    const void* q; /* heads may be 0: keys and values only */
+    const void* k;
+    const void* v;
+    void* q_out;
+    uint64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float* q_bias; /* [heads * head_dim], [kv_heads * head_dim] twice, or NULL: added before norm and rotation */
+    const float* k_bias;
+    const float* v_bias;
+    const float* q_norm; /* [head_dim] or NULL: each head over its root mean square (eps added to the mean), times this */
+    const float* k_norm;
+    const double* rope_turns; /* [rope_dim / 2] turns a position of every pair, from brisk_cuda_rope_turns            */
+    uint32_t rope_dim;        /* leading values of a head that rotate; 0: none                                        */
+    int32_t rope_adjacent;    /* 0: pairs (i, i + rope_dim / 2); 1: pairs (2 i, 2 i + 1)                              */
+    float rope_attn_factor;   /* cos and sin are multiplied by this; 0 means 1                                        */
+    float eps;
+    uint32_t heads;
+    int32_t type; /* of q, k, v and q_out: BRISK_TYPE_F32, _F16 or _BF16 */
+} brisk_cuda_cache4_rows;
+
+/* turns[i] = scale * base^(-2 i / rope_dim) / factors[i] / 2 pi for i < rope_dim / 2 (factors may be NULL), HOST pointers: what a program
+ * uploads once. Angles are made of them in 64 bits, so far positions rotate as exactly as near ones. */
+int brisk_cuda_rope_turns(uint32_t rope_dim, double base, double scale, const float* factors, double* turns, char* err, size_t errlen);
+
+/* Norms, rotates and hands back the queries; norms, rotates and stores the keys; stores the values, each at its position. */
+int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const brisk_cuda_cache4_batch* batch, const brisk_cuda_cache4_rows* rows, void* stream,
+                             char* err, size_t errlen);
+
+/* out[row][head] = sum over the positions j the row sees of softmax(scale * q . k_j) v_j: those up to its own, with a window only the last
+ * `window` of them (0: all). Query head h reads key/value head h / (heads / kv_heads). scale 0: 1 / sqrt(head_dim). A row that sees
+ * nothing is zeros. out may not be q. Sums and softmax statistics are held in 32 bits; with f32 queries products are as exact as 32 bits
+ * make them, with f16 and bf16 the probabilities are rounded to f16. */
+int brisk_cuda_cache4_attention(const brisk_cuda_cache4* cache, const brisk_cuda_cache4_batch* batch, int32_t type, const void* q, void* out, uint64_t q_stride,
+                                uint64_t out_stride, uint32_t heads, float scale, uint32_t window, void* stream, char* err, size_t errlen);
+
+/* The cached rows at the positions of the batch's tokens, as values of `type`: k and v are [tokens][kv_heads][head_dim] with the token
+ * strides given (a prefix handed to another program, a cache compared with another). context 0 and tokens = length reads all of one. */
+int brisk_cuda_cache4_read(const brisk_cuda_cache4* cache, const brisk_cuda_cache4_batch* batch, int32_t type, void* k, void* v, uint64_t k_stride, uint64_t v_stride,
+                           void* stream, char* err, size_t errlen);
+
 /* How single-token steps run in this session, as text: "persistent step kernel on: <configuration>" or
  * "persistent step kernel off: <reason>" (tensor parallel, flags, a model outside what the kernel covers or whose tokens
  * are all faster without it, a barrier that timed out earlier). The configuration ends with the positions at which tokens
