@@ -98,9 +98,6 @@ __device__ __forceinline__ int32_t page_of(const Cache4& c, const Cache4Batch& b
     return page >= 0 && uint32_t(page) < c.pages ? page : -1;
 }
 
-template <class T> __device__ __forceinline__ float widen(T v);
-template <> __device__ __forceinline__ float widen<float>(float v) { return v; }
-template <> __device__ __forceinline__ float widen<__half>(__half v) { return __half2float(v); }
 #endif
 
 }  // namespace bk
