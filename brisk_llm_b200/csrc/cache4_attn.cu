@@ -26,13 +26,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // an 8 x 8 matrix of f16, lane (g, t) holding row g, columns 2 t and 2 t + 1
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(v));
     return y;
 }
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
@@ -57,26 +62,57 @@ __device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4
     v[3] = bits(__hmul2(__hfma2(halves((u & 0x00f000f0u) | magic), sixteenth, less), scale));
 }
 
-template <int D> struct Split {
-    static constexpr int kTile = 32;                      // positions a warp takes at a time
-    static constexpr int kWarps = D == 256 ? 4 : 8;
+// The same eight numbers without a scale.
+__device__ __forceinline__ void centred(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t magic = 0x64006400u, u = w >> 8;
+    const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72
+    v[0] = bits(__hsub2(halves((w & 0x000f000fu) | magic), bias));
+    v[1] = bits(__hfma2(halves((w & 0x00f000f0u) | magic), sixteenth, less));
+    v[2] = bits(__hsub2(halves((u & 0x000f000fu) | magic), bias));
+    v[3] = bits(__hfma2(halves((u & 0x00f000f0u) | magic), sixteenth, less));
+}
+// The numbers n, not n - 8, as they are: four bits at the bottom of an f16 are n 2^-24, at bit 4 they are 16 n 2^-24, both exact.
+__device__ __forceinline__ void as_they_are(uint32_t w, uint32_t (&v)[4]) {
+    const uint32_t u = w >> 8;
+    v[0] = w & 0x000f000fu;
+    v[1] = w & 0x00f000f0u;
+    v[2] = u & 0x000f000fu;
+    v[3] = u & 0x00f000f0u;
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// W warps a CTA, 8 NT rows, f32 (two f16 parts) or not.
+template <int D, int NT, int W, bool TWO> struct Split {
+    static constexpr int kTile = 32;  // positions a warp takes at a time
+    static constexpr int kRows = 8 * NT, kThreads = 32 * W;
     static constexpr int kStages = D == 64 ? 4 : 3;
     static constexpr int kRow = D / 2, kScales = D / 16;  // bytes of a position
     static constexpr int kK = 0, kV = kTile * kRow, kKs = 2 * kTile * kRow, kVs = kKs + kTile * kScales, kStage = kVs + kTile * kScales;
-    static constexpr int kPitch = D + 4;                  // floats between two rows of a warp's result
+    static constexpr int kPitch = D + 4;  // floats between two rows of a warp's result
     static constexpr int kSteps = D / 16;
-    static constexpr size_t ring() { return size_t(kWarps) * kStages * kStage; }
-    static constexpr size_t parts(int nt) { return size_t(kWarps) * 8 * nt * kPitch * 4; }
-    static constexpr size_t body(int nt) { return ring() > parts(nt) ? ring() : parts(nt); }
-    static constexpr size_t queries(int nt, bool two) { return size_t(nt) * kSteps * 32 * 8 * (two ? 2 : 1); }
-    static constexpr size_t smem(int nt, bool two) { return body(nt) + queries(nt, two) + size_t(8 * nt) * (2 * kWarps + 4 + 16) * 4; }
+    static constexpr bool kHeld = NT == 1 && !TWO && D <= 128;  // the queries stay in registers
+    static constexpr size_t kRing = size_t(W) * kStages * kStage, kParts = size_t(W) * kRows * kPitch * 4;
+    // behind the loop, in the ring's place: the warps' results, this CTA's share of all CTAs', each warp's maximum, sum and factor and the
+    // CTAs' maxima and sums of each row
+    static constexpr size_t kJoining = kParts + size_t(kRows) * D * 4 + size_t(kRows) * (3 * W + 32) * 4;
+    static constexpr size_t kBody = kRing > kJoining ? kRing : kJoining;
+    static constexpr size_t kQueries = size_t(NT) * kSteps * 32 * 8 * (TWO ? 2 : 1);
+    // queries that go to registers pass through the last stage of the first warp, which the loop fills first
+    static constexpr size_t kQueriesAt = kHeld ? size_t(kStages - 1) * kStage : kBody;
+    static_assert(!kHeld || kQueries <= size_t(kStage));
+    static constexpr size_t kRowsAt = kBody + (kHeld ? 0 : kQueries), kBytes = kRowsAt + size_t(kRows) * (3 + D / 32) * 4;
+    // CTAs of an SM that registers and shared memory are meant for
+    static constexpr int kResident = D < 256 && (NT == 1 || (NT == 2 && D == 64)) ? 16 / W : W == 4 ? 2 : 1;
 };
 
 // Where 16 bytes of a position's row lie in a stage, and which position a row of a matrix instruction is: chosen so that the loads of
-// keys (8 rows, a quarter of each to a lane) and of values (4 rows, an eighth to a lane) meet no shared-memory bank twice.
+// keys (8 rows, 4 bytes of one block to a lane) and of values (4 rows, an eighth to a lane) meet no shared-memory bank twice.
 template <int D> __device__ __forceinline__ uint32_t chunk_of(uint32_t position, uint32_t chunk) {
-    if (D == 64) return chunk;
-    return D == 128 ? chunk ^ (((position >> 1) & 1) << 1) : chunk ^ ((position & 3) << 1);
+    if (D == 64) return chunk ^ ((position >> 2) & 1);
+    if (D == 128) return chunk ^ (((position >> 1) & 1) << 1) ^ ((position >> 2) & 1);
+    return chunk ^ ((position & 3) << 1) ^ ((position >> 2) & 1);
 }
 template <int D> __device__ __forceinline__ uint32_t position_of(uint32_t g) {  // g < 8
     return (g & 1) ? 4 + ((g >> 1) ^ (D == 128 ? 1 : 2)) : g >> 1;
@@ -89,19 +125,23 @@ template <int D> __device__ __forceinline__ uint32_t position_of(uint32_t g) {  
 // so that eight query heads fill an instruction and the 4-bit words become its A operand in registers, straight from the
 // stage that cp.async filled: any order of the head's values does for K Q^T as long as Q has the same. P^T is S^T transposed in the warp.
 // f32 queries and weights are two f16 parts each (22 bits); others one.
-template <class T, int D, int NT>
-__global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && D == 64) ? 2 : 1) cache4_split_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a) {
-    using G = Split<D>;
+template <class T, int D, int NT, int W>
+__global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResident) cache4_split_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a) {
     constexpr bool kTwo = sizeof(T) == 4;
-    constexpr int kRows = 8 * NT, kThreads = G::kWarps * 32;
+    using G = Split<D, NT, W, kTwo>;
+    constexpr int kRows = G::kRows, kThreads = G::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char* q_frag = smem + G::body(NT);
-    float* row_scale = reinterpret_cast<float*>(q_frag + G::queries(NT, kTwo));  // [kRows]
-    float* warp_top = row_scale + kRows;                                         // [kWarps][kRows], then the sums
-    float* warp_sum_ = warp_top + G::kWarps * kRows;
-    float* cta_top = warp_sum_ + G::kWarps * kRows;  // [kRows], read by the cluster
-    float* cta_sum = cta_top + kRows;
-    float* weight = cta_sum + kRows;  // [16][kRows]
+    unsigned char* q_frag = smem + G::kQueriesAt;
+    float* row_scale = reinterpret_cast<float*>(smem + G::kRowsAt);  // [kRows]
+    int* row_last = reinterpret_cast<int*>(row_scale + kRows);       // [kRows] the last position a row sees
+    int* row_first = row_last + kRows;                               // [kRows] and the first
+    float* offset = reinterpret_cast<float*>(row_first + kRows);     // [D / 32][kRows]
+    float* received = reinterpret_cast<float*>(smem + G::kParts);    // [S][kRows D / S]: this CTA's share of every CTA's result
+    float* warp_top = received + kRows * D;                          // [W][kRows]
+    float* warp_total = warp_top + W * kRows;
+    float* factor = warp_total + W * kRows;
+    float* tops = factor + W * kRows;  // [16][kRows], of the cluster's CTAs
+    float* totals = tops + 16 * kRows;
 
     wait_for_previous();
     cg::cluster_group cluster = cg::this_cluster();
@@ -109,60 +149,23 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t unit = blockIdx.x / S, kv = unit % c.kv_heads, tile = unit / c.kv_heads, sequence = blockIdx.y;
     const uint32_t group = a.heads / c.kv_heads;
+    const long long context = b.context[sequence];
     uint32_t first_row, count;
     sequence_rows(b, sequence, first_row, count);
     const uint32_t total = count * group, row0 = tile * kRows;
     if (row0 >= total) return;  // the whole cluster
     const uint32_t rows = min(total - row0, uint32_t(kRows));
-    const long long context = b.context[sequence], held = (long long)b.columns * c.page_size;
-    const long long first_pos = context + row0 / group, last_pos = context + (row0 + rows - 1) / group;
-    const int hi = int(min(last_pos, held - 1));  // -1 and less: nothing
-    const int lo = a.window != 0 ? int(min(max(first_pos - (long long)a.window + 1, 0ll), held)) : 0;
-
-    // ---- queries: a power of two brings a row's largest value to 2^10, so that bf16 and both parts of f32 fit f16 ----
-    for (uint32_t r = warp; r < kRows; r += G::kWarps) {
-        float x[D / 32], most = 0.0f;
-        const T* src = static_cast<const T*>(a.q) + size_t(first_row + (row0 + r) / group) * a.q_stride + size_t(kv * group + (row0 + r) % group) * D;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            x[j] = r < rows ? to_float(src[lane + 32 * j]) : 0.0f;
-            most = fmaxf(most, fabsf(x[j]));
-        }
-        most = warp_max(most);
-        const int up = most > 0.0f && most < INFINITY ? 10 - ilogbf(most) : 0;
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-            const float v = ldexpf(a.scale < 0.0f ? -x[j] : x[j], up);
-            const __half high = __float2half_rn(v);
-            // value `lane` of block j: which lane's fragment of which step takes it (see widen and the loads of keys below)
-            const uint32_t byte = lane & 15, word = byte >> 2;
-            const uint32_t owner = D == 64 ? j * 2 + (word >> 1) : j & 3;
-            const uint32_t step = (D == 64 ? 2 * (word & 1) : D == 128 ? 2 * word : (j >> 2) * 8 + 2 * word) + (byte & 1);
-            const uint32_t at = ((((r >> 3) * G::kSteps + step) * 32 + (r & 7) * 4 + owner) * 2 + (lane >> 4)) * 2 + ((byte & 3) >> 1);
-            __half* dst = reinterpret_cast<__half*>(q_frag);
-            dst[at] = high;
-            if (kTwo) dst[at + NT * G::kSteps * 128] = __float2half_rn(v - __half2float(high));
-        }
-        if (lane == 0) row_scale[r] = ldexpf(fabsf(a.scale) * 1.4426950408889634f, -up);
-    }
-    __syncthreads();
-
-    float o[G::kSteps][NT][4], m[NT][2], l[NT][2], scale[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < G::kSteps; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            m[n][e] = -INFINITY;
-            l[n][e] = 0.0f;
-            scale[n][e] = row_scale[n * 8 + 2 * t + e];
-        }
-    }
+    // the positions that a token of the sequence sees; last < first: none
+    const long long held = (long long)b.columns * c.page_size;
+    auto last_of = [&](uint32_t token) { return int(max(min(context + token, held - 1), -1ll)); };
+    auto first_of = [&](uint32_t token) { return a.window != 0 ? int(min(max(context + token - (long long)a.window + 1, 0ll), held)) : 0; };
+    const uint32_t token0 = row0 / group, token1 = (row0 + rows - 1) / group;
+    const int lo = first_of(token0), hi = last_of(token1);
+    const int whole_from = first_of(token1), whole_to = last_of(token0);  // what every row sees
 
     // ---- the warp's tiles: begin + 32 (rank + S (warp + W i)) and on ----
     const int begin = lo & ~31;
-    const int tiles = hi >= lo ? (hi - begin) / 32 + 1 : 0, stride = int(S) * G::kWarps, mine = int(warp * S + rank);
+    const int tiles = hi >= lo ? (hi - begin) / 32 + 1 : 0, stride = int(S) * W, mine = int(warp * S + rank);
     unsigned char* ring = smem + size_t(warp) * G::kStages * G::kStage;
     const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring));
     // lanes 0 and 1 know the pages of the tile's two halves, asked for a tile ahead of the copies
@@ -208,7 +211,67 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
         page_next = page_for(mine + (s + 1) * stride);
         request(mine + s * stride, page, s);
     }
+    // ---- queries: a power of two brings a row's largest value to 2^10, so that bf16 and both parts of f32 fit f16. For f16 and bf16 the
+    // keys' numbers are used as they are: values that meet the high four bits of a byte are a sixteenth, and the -8 of a block's numbers is
+    // -8 times the sum of its queries, where the sum begins. That takes a third of the instructions and, as the sums cancel, two bits of
+    // 32-bit sums that f32 queries would miss: theirs are n - 8. ----
+    for (uint32_t r = warp; r < kRows; r += W) {
+        float x[D / 32], most = 0.0f;
+        const uint32_t token = (row0 + r) / group, head = (row0 + r) - token * group;
+        const T* src = static_cast<const T*>(a.q) + size_t(first_row + token) * a.q_stride + size_t(kv * group + head) * D;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            x[j] = r < rows ? to_float(src[lane + 32 * j]) : 0.0f;
+            most = fmaxf(most, fabsf(x[j]));
+        }
+        most = warp_max(most);
+        const int exponent = int(__float_as_uint(most) >> 23) - 127, up = most < INFINITY ? min(10 - exponent, 100) : 0;
+        const uint32_t byte = lane & 15;
+        const bool sixteenth = !kTwo && lane >= 16;
+        const float by = __uint_as_float(uint32_t(127 + up - (sixteenth ? 4 : 0)) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+            const float v = x[j] * by;
+            const __half high = __float2half_rn(v);
+            const uint32_t step = 2 * j + (byte & 1), at = ((((r >> 3) * G::kSteps + step) * 32 + (r & 7) * 4 + (byte >> 2)) * 2 + (lane >> 4)) * 2 + ((byte >> 1) & 1);
+            __half* dst = reinterpret_cast<__half*>(q_frag);
+            dst[at] = high;
+            if (kTwo) {
+                dst[at + NT * G::kSteps * 128] = __float2half_rn(v - __half2float(high));
+            } else {
+                const float sum = warp_sum(__half2float(high) * (sixteenth ? 16.0f : 1.0f));
+                if (lane == 0) offset[j * kRows + r] = sum * -0x1p-21f;  // -8 times it, in units of 2^-24
+            }
+        }
+        if (lane == 0) {
+            row_scale[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 - up) << 23) * (kTwo ? 1.0f : 0x1p24f);
+            row_last[r] = last_of(token);
+            row_first[r] = first_of(token);
+        }
+    }
+    __syncthreads();
+
+    float o[G::kSteps][NT][4], m[NT][2], l[NT][2], scale[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < G::kSteps; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[n][e] = -INFINITY;
+            l[n][e] = 0.0f;
+            scale[n][e] = row_scale[n * 8 + 2 * t + e];
+        }
+    }
+
     const uint2* frag = reinterpret_cast<const uint2*>(q_frag) + lane;
+    constexpr bool kHeld = G::kHeld;
+    uint2 held_q[kHeld ? G::kSteps : 1];
+    if (kHeld) {
+#pragma unroll
+        for (int i = 0; i < G::kSteps; ++i) held_q[kHeld ? i : 0] = frag[i * 32];
+        __syncthreads();
+    }
     uint32_t slot = 0;
     for (int j = mine; j < tiles; j += stride) {
         {
@@ -227,46 +290,51 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
 #pragma unroll
             for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.0f;
             const uint32_t pa = 16 * h + position_of<D>(g), pb = pa + 8;
+            constexpr int kBlocks = D / 32;
+            float da[kBlocks], db[kBlocks];
 #pragma unroll
-            for (int part = 0; part < (D == 256 ? 2 : 1); ++part) {
-                constexpr int kWords = D == 64 ? 2 : 4;
-                uint32_t wa[kWords], wb[kWords];
-                const uint32_t block = D == 64 ? t >> 1 : part * 4 + t;
-                if (D == 64) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(st + G::kK + pa * G::kRow + t * 8), y = *reinterpret_cast<const uint2*>(st + G::kK + pb * G::kRow + t * 8);
-                    wa[0] = x.x; wa[1] = x.y; wb[0] = y.x; wb[1] = y.y;
+            for (int i = 0; i < kBlocks / 2; ++i) {
+                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(st + G::kKs + pa * G::kScales + i * 4));
+                const float2 y = __half22float2(*reinterpret_cast<const __half2*>(st + G::kKs + pb * G::kScales + i * 4));
+                da[2 * i] = x.x; da[2 * i + 1] = x.y;
+                db[2 * i] = y.x; db[2 * i + 1] = y.y;
+            }
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) {
+                uint32_t va[4], vb[4];
+                const uint32_t wa = *reinterpret_cast<const uint32_t*>(st + G::kK + pa * G::kRow + chunk_of<D>(pa, k) * 16 + t * 4);
+                const uint32_t wb = *reinterpret_cast<const uint32_t*>(st + G::kK + pb * G::kRow + chunk_of<D>(pb, k) * 16 + t * 4);
+                if (kTwo) {
+                    centred(wa, va);
+                    centred(wb, vb);
                 } else {
-                    const uint4 x = *reinterpret_cast<const uint4*>(st + G::kK + pa * G::kRow + chunk_of<D>(pa, block) * 16);
-                    const uint4 y = *reinterpret_cast<const uint4*>(st + G::kK + pb * G::kRow + chunk_of<D>(pb, block) * 16);
-                    wa[0] = x.x; wa[1] = x.y; wa[kWords - 2] = x.z; wa[kWords - 1] = x.w;
-                    wb[0] = y.x; wb[1] = y.y; wb[kWords - 2] = y.z; wb[kWords - 1] = y.w;
+                    as_they_are(wa, va);
+                    as_they_are(wb, vb);
                 }
-                const __half2 da = __half2half2(*reinterpret_cast<const __half*>(st + G::kKs + pa * G::kScales + block * 2));
-                const __half2 db = __half2half2(*reinterpret_cast<const __half*>(st + G::kKs + pb * G::kScales + block * 2));
 #pragma unroll
-                for (int w = 0; w < kWords; ++w) {
-                    uint32_t va[4], vb[4];
-                    widen(wa[w], da, va);
-                    widen(wb[w], db, vb);
+                for (int n = 0; n < NT; ++n) {
+                    const float2 begin_at = kTwo ? make_float2(0.0f, 0.0f) : *reinterpret_cast<const float2*>(offset + k * kRows + n * 8 + 2 * t);
+                    float y[4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int step = part * 8 + 2 * w + u;
-                            const uint2 q = frag[(n * G::kSteps + step) * 32];
-                            mma16816(s[h][n], va[2 * u], vb[2 * u], va[2 * u + 1], vb[2 * u + 1], q.x, q.y);
-                            if (kTwo) {
-                                const uint2 r = frag[((NT + n) * G::kSteps + step) * 32];
-                                mma16816(s[h][n], va[2 * u], vb[2 * u], va[2 * u + 1], vb[2 * u + 1], r.x, r.y);
-                            }
+                    for (int u = 0; u < 2; ++u) {
+                        const uint2 q = kHeld ? held_q[kHeld ? 2 * k + u : 0] : frag[(n * G::kSteps + 2 * k + u) * 32];
+                        if (u == 0) mma16816(y, va[0], vb[0], va[1], vb[1], q.x, q.y, begin_at.x, begin_at.y);
+                        else mma16816(y, va[2], vb[2], va[3], vb[3], q.x, q.y);
+                        if (kTwo) {
+                            const uint2 r = frag[((NT + n) * G::kSteps + 2 * k + u) * 32];
+                            mma16816(y, va[2 * u], vb[2 * u], va[2 * u + 1], vb[2 * u + 1], r.x, r.y);
                         }
                     }
+                    s[h][n][0] = fmaf(y[0], da[k], s[h][n][0]);
+                    s[h][n][1] = fmaf(y[1], da[k], s[h][n][1]);
+                    s[h][n][2] = fmaf(y[2], db[k], s[h][n][2]);
+                    s[h][n][3] = fmaf(y[3], db[k], s[h][n][3]);
                 }
             }
         }
 
         // scores in powers of two, hidden ones to -inf
-        const bool whole = base + 31 <= first_pos && base + 31 <= hi && (a.window == 0 || (long long)base > last_pos - (long long)a.window);
+        const bool whole = base + 31 <= whole_to && base >= whole_from;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -277,14 +345,13 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
             if (!whole) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const long long at = context + (row0 + n * 8 + 2 * t + e) / group;
+                    const int last = row_last[n * 8 + 2 * t + e], first = row_first[n * 8 + 2 * t + e];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const int p = base + 16 * h + 8 * u + int(position_of<D>(g));
-                            const bool seen = p <= at && p <= hi && (a.window == 0 || p > at - (long long)a.window);
-                            if (!seen) s[h][n][2 * u + e] = -INFINITY;
+                            if (p > last || p < first) s[h][n][2 * u + e] = -INFINITY;
                         }
                     }
                 }
@@ -355,7 +422,7 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
             for (int i = 0; i < 4; ++i) {
                 const unsigned char* row = st + G::kV + pos[i] * G::kRow;
                 if (D == 64) {
-                    w[i][0] = *reinterpret_cast<const uint32_t*>(row + g * 4);
+                    w[i][0] = *reinterpret_cast<const uint32_t*>(row + chunk_of<D>(pos[i], g >> 2) * 16 + (g & 3) * 4);
                 } else if (D == 128) {
                     const uint2 x = *reinterpret_cast<const uint2*>(row + chunk_of<D>(pos[i], g >> 1) * 16 + (g & 1) * 8);
                     w[i][0] = x.x; w[i][kWords - 1] = x.y;
@@ -363,8 +430,14 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
                     const uint4 x = *reinterpret_cast<const uint4*>(row + chunk_of<D>(pos[i], g) * 16);
                     w[i][0] = x.x; w[i][1 % kWords] = x.y; w[i][2 % kWords] = x.z; w[i][kWords - 1] = x.w;
                 }
-                const int p = base + int(pos[i]);
-                d[i] = p >= lo && p <= hi ? *reinterpret_cast<const __half*>(st + G::kVs + pos[i] * G::kScales + block * 2) : __half(0.0f);
+                d[i] = *reinterpret_cast<const __half*>(st + G::kVs + pos[i] * G::kScales + block * 2);
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int p = base + int(pos[i]);
+                    if (p < lo || p > hi) d[i] = __half(0.0f);
+                }
             }
             const __half2 d0 = __halves2half2(d[0], d[1]), d1 = __halves2half2(d[2], d[3]);
 #pragma unroll
@@ -392,6 +465,7 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
     copies_wait<0>();
     release_next();
     __syncthreads();  // the rings become the warps' results
+    if (S > 1) cluster_arrive();  // waited for before anything is written into another CTA's
 
     // ---- join ----
     float* part = reinterpret_cast<float*>(smem) + size_t(warp) * kRows * G::kPitch;
@@ -406,7 +480,7 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
             const uint32_t r = n * 8 + 2 * t + e;
             if (g == 0) {
                 warp_top[warp * kRows + r] = m[n][e];
-                warp_sum_[warp * kRows + r] = x;
+                warp_total[warp * kRows + r] = x;
             }
 #pragma unroll
             for (int i = 0; i < G::kSteps; ++i) {  // value f = (2 i + upper) 8 + g of the row is dim (B / 16) 32 + B % 16 + 16 upper, B = g D / 16 + i
@@ -416,50 +490,81 @@ __global__ void __launch_bounds__(Split<D>::kWarps * 32, NT == 1 || (NT == 2 && 
         }
     }
     __syncthreads();
-    for (uint32_t x = tid; x < uint32_t(G::kWarps * kRows); x += kThreads) {  // warp_top becomes each warp's factor
-        const uint32_t r = x % kRows;
-        float most = -INFINITY;
-        for (int w = 0; w < G::kWarps; ++w) most = fmaxf(most, warp_top[w * kRows + r]);
-        const float mine_top = warp_top[x];
-        weight[x] = mine_top == -INFINITY ? 0.0f : exp2_fast(mine_top - most);
-        if (x < kRows) cta_top[r] = most;
-    }
-    __syncthreads();
-    if (tid < kRows) {
-        float sum = 0.0f;
-        for (int w = 0; w < G::kWarps; ++w) sum = fmaf(warp_sum_[w * kRows + tid], weight[w * kRows + tid], sum);
-        cta_sum[tid] = sum;
-    }
-    float* joined = reinterpret_cast<float*>(smem);
-    for (uint32_t x = tid; x < uint32_t(kRows * D); x += kThreads) {
-        const uint32_t at = (x / D) * G::kPitch + x % D;
-        float sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < G::kWarps; ++w) sum = fmaf(joined[size_t(w) * kRows * G::kPitch + at], weight[w * kRows + x / D], sum);
-        joined[at] = sum;  // of its own value only: no other thread reads it here
-    }
-    if (S > 1) cluster.sync();
-    else __syncthreads();
-    // the CTAs' factors over the sum of all
     if (tid < kRows) {
         float most = -INFINITY, sum = 0.0f;
-        for (uint32_t k = 0; k < S; ++k) most = fmaxf(most, *cluster.map_shared_rank(cta_top + tid, k));
+#pragma unroll
+        for (int w = 0; w < W; ++w) most = fmaxf(most, warp_top[w * kRows + tid]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float top = warp_top[w * kRows + tid], x = top == -INFINITY ? 0.0f : exp2_fast(top - most);
+            factor[w * kRows + tid] = x;
+            sum = fmaf(warp_total[w * kRows + tid], x, sum);
+        }
+        if (S == 1) row_scale[tid] = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+        tops[rank * kRows + tid] = most;
+        totals[rank * kRows + tid] = sum;
+    }
+    __syncthreads();
+    // value f of a row is this dim of the head (see above)
+    auto dim_of = [](uint32_t f) {
+        const uint32_t B = (f & 7) * (D / 16) + (f >> 4);
+        return (B >> 4) * 32 + (B & 15) + ((f >> 3) & 1) * 16;
+    };
+    auto row_of = [&](uint32_t r) {
+        const uint32_t token = (row0 + r) / group;
+        return static_cast<T*>(a.out) + size_t(first_row + token) * a.out_stride + size_t(kv * group + (row0 + r) - token * group) * D;
+    };
+    // Where a cluster has several CTAs each sums a share of the values: the others write theirs into it, then all meet once.
+    const uint32_t share_log = 31 - __clz(uint32_t(kRows * D)) - (31 - __clz(S)), share = 1u << share_log;
+    if (S > 1) cluster_wait();
+    for (uint32_t r = warp; r < kRows; r += W) {
+        if (S == 1 && r >= rows) break;
+        float by[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w) by[w] = factor[w * kRows + r];
+        T* out = row_of(r);
+        const float scale_r = S == 1 ? row_scale[r] : 1.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const uint32_t f = i * 32 + lane;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) sum = fmaf(reinterpret_cast<const float*>(smem)[(w * kRows + r) * G::kPitch + f], by[w], sum);
+            if (S == 1) {
+                put(out + dim_of(f), sum * scale_r);
+            } else {
+                const uint32_t x = r * D + f;
+                *cluster.map_shared_rank(received + rank * share + (x & (share - 1)), x >> share_log) = sum;
+            }
+        }
+    }
+    if (S == 1) return;
+    for (uint32_t x = tid; x < kRows * S; x += kThreads) {
+        const uint32_t r = x % kRows, k = x / kRows;
+        if (k != rank) {
+            *cluster.map_shared_rank(tops + rank * kRows + r, k) = tops[rank * kRows + r];
+            *cluster.map_shared_rank(totals + rank * kRows + r, k) = totals[rank * kRows + r];
+        }
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (tid < kRows) {
+        float most = -INFINITY, sum = 0.0f;
+        for (uint32_t k = 0; k < S; ++k) most = fmaxf(most, tops[k * kRows + tid]);
         for (uint32_t k = 0; k < S; ++k) {
-            const float top = *cluster.map_shared_rank(cta_top + tid, k), w = top == -INFINITY ? 0.0f : exp2_fast(top - most);
-            sum = fmaf(*cluster.map_shared_rank(cta_sum + tid, k), w, sum);
-            weight[k * kRows + tid] = w;
+            const float top = tops[k * kRows + tid], x = top == -INFINITY ? 0.0f : exp2_fast(top - most);
+            sum = fmaf(totals[k * kRows + tid], x, sum);
+            tops[k * kRows + tid] = x;  // now its factor
         }
         row_scale[tid] = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
     }
     __syncthreads();
-    for (uint32_t x = rank * kThreads + tid; x < rows * D; x += S * kThreads) {
-        const uint32_t r = x / D, f = x % D, at = r * G::kPitch + f;
+    for (uint32_t x = tid; x < share; x += kThreads) {
+        const uint32_t r = (rank * share + x) / D;
         float sum = 0.0f;
-        for (uint32_t k = 0; k < S; ++k) sum = fmaf(*cluster.map_shared_rank(joined + at, k), weight[k * kRows + r], sum);
-        const uint32_t B = (f & 7) * (D / 16) + (f >> 4), dim = (B >> 4) * 32 + (B & 15) + ((f >> 3) & 1) * 16;
-        put(static_cast<T*>(a.out) + size_t(first_row + (row0 + r) / group) * a.out_stride + size_t(kv * group + (row0 + r) % group) * D + dim, sum * row_scale[r]);
+        for (uint32_t k = 0; k < S; ++k) sum = fmaf(received[k * share + x], tops[k * kRows + r], sum);
+        if (r < rows) put(row_of(r) + dim_of((rank * share + x) % D), sum * row_scale[r]);
     }
-    if (S > 1) cluster.sync();  // nobody leaves while its shared memory is read
 }
 
 uint32_t multiprocessors() {
@@ -468,27 +573,20 @@ uint32_t multiprocessors() {
     return uint32_t(count);
 }
 
-template <class T, int D, int NT>
-void attend_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, bool dependent, cudaStream_t s) {
-    using G = Split<D>;
-    const auto kernel = cache4_split_kernel<T, D, NT>;
-    constexpr size_t smem = G::smem(NT, sizeof(T) == 4);
-    static_assert(smem <= 227 * 1024);
+template <class T, int D, int NT, int W>
+void launch_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, uint64_t units, uint32_t split, bool dependent, cudaStream_t s) {
+    using G = Split<D, NT, W, sizeof(T) == 4>;
+    const auto kernel = cache4_split_kernel<T, D, NT, W>;
+    static_assert(G::kBytes <= 227 * 1024);
     static DeviceOnce once;
     if (once.first()) {
-        BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+        BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(G::kBytes)));
         BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     }
-    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
-    const uint64_t units = tiles * c.kv_heads * b.sequences;
-    const uint64_t length = a.window != 0 ? std::min<uint64_t>(b.max_length, uint64_t(a.window) + 8 * NT + 31) : b.max_length;
-    uint32_t split = 1;
-    while (split < 16 && units * split < 2 * multiprocessors() && length > uint64_t(split) * G::kWarps * 64) split *= 2;
-    if (units / b.sequences * split > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(uint32_t(units / b.sequences * split), b.sequences);
-    cfg.blockDim = dim3(G::kWarps * 32);
-    cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = dim3(32 * W);
+    cfg.dynamicSmemBytes = G::kBytes;
     cfg.stream = s;
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -499,6 +597,23 @@ void attend_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, 
     cfg.attrs = attr;
     cfg.numAttrs = dependent ? 2 : 1;
     BK_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, b, a));
+}
+
+template <class T, int D, int NT>
+void attend_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, bool dependent, cudaStream_t s) {
+    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
+    const uint64_t units = tiles * c.kv_heads * b.sequences;
+    const uint64_t length = a.window != 0 ? std::min<uint64_t>(b.max_length, uint64_t(a.window) + 8 * NT + 31) : b.max_length;
+    // Clusters grow while there are CTAs to spare (two to an SM for up to 8 rows; those of more rows, with an SM's shared memory to
+    // themselves, to half the SMs, past which clusters wait for room) and a tile for every warp. us at S = 1, 2, 4, 8, 16: one token
+    // of 8 key/value heads at 517 positions 8.0 7.8 6.5 6.5 7.5, at 32 767 192 107 56 33 27, of 64 x 8 at 8000 107 106 117 165 297; 36 rows
+    // of 8 heads at 2064 44 30 21 31 37. Four or sixteen warps a CTA are no faster at any of them.
+    constexpr int kWarps = D == 256 ? 4 : 8;
+    const uint64_t most = NT == 1 ? 2 * multiprocessors() : multiprocessors() / 2;
+    uint32_t split = 1;
+    while (split < 16 && units * split * 2 <= most && length > uint64_t(split) * kWarps * 32) split *= 2;
+    if (units / b.sequences * split > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
+    launch_split<T, D, NT, kWarps>(c, b, a, units, split, dependent, s);
 }
 
 template <class T, int D>
