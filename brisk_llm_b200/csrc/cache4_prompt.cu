@@ -1,0 +1,575 @@
+// Attention over the paged cache in 4 bits for many rows - prompts and their chunks - on the tensor cores of tensor memory.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "cache4.h"
+#include "packed.cuh"
+#include "pdl.cuh"
+#include "tc.cuh"
+
+namespace bk {
+namespace {
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// The eight numbers of a word, n - 8 times the scale, as four pairs: (low of bytes 0, 2), (high of 0, 2), (low of 1, 3), (high of 1, 3);
+// exact (see cache4_attn.cu).
+__device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4]) {
+    const uint32_t magic = 0x64006400u, u = w >> 8;
+    const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72
+    v[0] = bits(__hmul2(__hsub2(halves((w & 0x000f000fu) | magic), bias), scale));
+    v[1] = bits(__hmul2(__hfma2(halves((w & 0x00f000f0u) | magic), sixteenth, less), scale));
+    v[2] = bits(__hmul2(__hsub2(halves((u & 0x000f000fu) | magic), bias), scale));
+    v[3] = bits(__hmul2(__hfma2(halves((u & 0x00f000f0u) | magic), sixteenth, less), scale));
+}
+
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+// 2^x of a pair without the special-function unit, which the weights of two tiles would keep busier than their products keep the
+// tensor cores: the integer part by adding 1.5 x 2^23, 2^r for r in [-1/2, 1/2] by the polynomial of degree 4 with the least
+// relative error (Remez: 2.6e-6, a hundredth of what rounding the weight to f16 costs), the integer into the exponent.
+__device__ __forceinline__ void exp2_by_polynomial(f32x2 x, float& y, float& z) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const f32x2 magic = pack2(12582912.0f, 12582912.0f), t = add2(x, magic), r = sub2(x, sub2(t, magic));
+    f32x2 p = fma2(r, pack2(0.0095701f, 0.0095701f), pack2(0.05591786f, 0.05591786f));
+    p = fma2(p, r, pack2(0.24024745f, 0.24024745f));
+    p = fma2(p, r, pack2(0.69312181f, 0.69312181f));
+    p = fma2(p, r, pack2(0.99999926f, 0.99999926f));
+    float ta, tb, pa, pb;
+    unpack2(t, ta, tb);
+    unpack2(p, pa, pb);
+    y = __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa));
+    z = __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb));
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"(uint32_t(accumulate)) : "memory");
+}
+// A in tensor memory: lane = row, a column holds two values of K
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t instr, bool accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(instr), "r"(uint32_t(accumulate)) : "memory");
+}
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+          "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+                   "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+                 : "r"(at)
+                 : "memory");
+}
+
+// A whole row, zeros where there is none: every load is under way before the first value is looked at.
+template <class T, int D> struct Row {
+    static constexpr int kPer = 16 / sizeof(T);
+    uint4 raw[D / kPer];
+    __device__ __forceinline__ void load(const T* p, bool there, int wide) {
+        if (!there) {
+#pragma unroll
+            for (int i = 0; i < D / kPer; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+        } else if (wide) {
+#pragma unroll
+            for (int i = 0; i < D / kPer; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < D / kPer; ++i) {
+                alignas(16) T y[kPer];
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) y[u] = p[i * kPer + u];
+                raw[i] = *reinterpret_cast<const uint4*>(y);
+            }
+        }
+    }
+    __device__ __forceinline__ float operator[](int i) const { return to_float(reinterpret_cast<const T*>(raw)[i]); }
+};
+
+template <int D, bool TWO> struct Prompt {
+    static constexpr int kN = TWO ? 64 : 128;  // positions of a tile
+    static constexpr int kParts = TWO ? 2 : 1;  // f16 parts of a query and of a weight
+    static constexpr int kPanel = 128 * 128;    // 128 rows of 128 bytes
+    static constexpr int kQ = D / 64 * kPanel;  // of one part of a query tile
+    static constexpr int kK = D / 64 * kN * 128, kV = kN / 64 * D * 128;
+    static constexpr int kKAt = 2 * kParts * kQ, kVAt = kKAt + 2 * kK, kBarriersAt = kVAt + 2 * kV;
+    static constexpr int kBytes = kBarriersAt + 256 + 1024;  // the tiles start on a 1024-byte boundary
+    // columns of tensor memory: a tile's scores, its weights (over the scores where they are one part), its result
+    static constexpr int kS = 128, kW = TWO ? 64 : 0, kO = 256;
+};
+constexpr int kByPolynomial = 1;  // of four pairs
+constexpr int kPromptThreads = 16 * 32;
+template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+struct Bars {
+    uint64_t q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full, drained;
+    uint32_t tmem;
+};
+
+// softmax(q k) v for 256 rows (or 128) - tokens times the query heads of one key/value head - of one sequence, in two tiles of 128 rows that
+// take turns on the tensor cores. Four warpgroups: one for each tile's softmax, a thread to a row (its maximum and sum need no other); one
+// widens the 4-bit keys and values of 128 positions (64 where queries are two f16 parts) into the operand tiles of the products,
+// once for both tiles of rows; a warp of the last issues the products,
+//     S = Q K^T (both operands in shared memory),     O += P V (P in tensor memory, where the softmax wrote it over S).
+// The head's values lie in Q and K in the order in which a 4-bit word yields them. V is widened with neighbouring positions side by side, as
+// the product wants them: two words of two positions give pairs of one dim.
+// Every wait is bounded; one that runs out leaves NaN in the rows of its tile.
+template <class T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a, uint32_t rows_per_cta) {
+    constexpr bool kTwo = sizeof(T) == 4;
+    using G = Prompt<D, kTwo>;
+    constexpr int kN = G::kN;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024 - (saddr(smem_raw) & 1023)) & 1023);
+    const uint32_t smem_at = saddr(smem);
+    Bars* bar = reinterpret_cast<Bars*>(smem + G::kBarriersAt);
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    wait_for_previous();
+    const uint32_t group = a.heads / c.kv_heads, sequence = blockIdx.y, kv = blockIdx.x % c.kv_heads;
+    const uint32_t tile = gridDim.x / c.kv_heads - 1 - blockIdx.x / c.kv_heads;  // the last rows, which see most, begin first
+    const long long context = b.context[sequence], held = (long long)b.columns * c.page_size;
+    uint32_t first_row, count;
+    sequence_rows(b, sequence, first_row, count);
+    const uint32_t total = count * group, row0 = tile * rows_per_cta;
+    const uint32_t rows = row0 < total ? min(total - row0, rows_per_cta) : 0;
+    if (rows == 0) return;
+    if (warp == 12) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&bar->q_full[i], 4);
+                mbar_init(&bar->k_full[i], 4);
+                mbar_init(&bar->k_free[i], 1);
+                mbar_init(&bar->v_full[i], 4);
+                mbar_init(&bar->v_free[i], 1);
+                mbar_init(&bar->s_full[i], 1);
+                mbar_init(&bar->p_full[i], 4);
+            }
+            mbar_init(&bar->o_full, 1);
+            mbar_init(&bar->drained, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(saddr(&bar->tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bar->tmem;
+
+    auto last_of = [&](uint32_t token) { return int(max(min(context + token, held - 1), -1ll)); };
+    auto first_of = [&](uint32_t token) { return a.window != 0 ? int(min(max(context + token - (long long)a.window + 1, 0ll), held)) : 0; };
+    const int lo = first_of(row0 / group), hi = last_of((row0 + rows - 1) / group);
+    const int begin = lo & ~(kN - 1), tiles = hi >= lo ? (hi - begin) / kN + 1 : 0, halves_used = rows > 128 ? 2 : 1;
+    const long long limit = kTcWaitCycles;
+    bool dead = false;
+
+    if (warp < 8) {
+        // ---- softmax: a thread to a row ----
+        more_registers<192>();
+        const uint32_t half = warp >> 2, r = tid & 127, row = row0 + half * 128 + r;
+        const bool real = half * 128 + r < rows;
+        const uint32_t token = real ? row / group : 0, head = row - token * group;
+        T* out = static_cast<T*>(a.out) + size_t(first_row + token) * a.out_stride + size_t(kv * group + head) * D;
+        if (int(half) < halves_used && tiles != 0) {
+            // the row's queries: a power of two brings the largest to 2^10 (see cache4_attn.cu)
+            Row<T, D> q;
+            q.load(static_cast<const T*>(a.q) + size_t(first_row + token) * a.q_stride + size_t(kv * group + head) * D, real, a.wide);
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D; ++i) most = fmaxf(most, fabsf(q[i]));
+            const int exponent = int(__float_as_uint(most) >> 23) - 127, up = most < INFINITY ? min(10 - exponent, 100) : 0;
+            const float by = __uint_as_float(uint32_t(127 + up) << 23) * (a.scale < 0.0f ? -1.0f : 1.0f);
+            const float scale = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 - up) << 23);
+            unsigned char* q_tile = smem + half * G::kParts * G::kQ;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {  // 16 bytes: the order of word u (see widen)
+                    uint32_t high[4], low[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int dim = u * 4 + (i >> 1) + (i & 1) * 16;
+                        const float y = q[k * 32 + dim] * by, z = q[k * 32 + dim + 2] * by;
+                        const __half2 h = __floats2half2_rn(y, z);
+                        high[i] = bits(h);
+                        if (kTwo) low[i] = bits(__floats2half2_rn(y - __low2float(h), z - __high2float(h)));
+                    }
+                    unsigned char* dst = q_tile + (k >> 1) * G::kPanel + r * 128 + ((((k & 1) * 4 + u) ^ (r & 7)) * 16);
+                    *reinterpret_cast<uint4*>(dst) = make_uint4(high[0], high[1], high[2], high[3]);
+                    if (kTwo) *reinterpret_cast<uint4*>(dst + G::kQ) = make_uint4(low[0], low[1], low[2], low[3]);
+                }
+            }
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->q_full[half]);
+
+            const int last = real ? last_of(token) : -1, first = real ? first_of(token) : 0;
+            const uint32_t last_row = min(row0 + half * 128 + 127, row0 + rows - 1);
+            const int whole_to = last_of((row0 + half * 128) / group), whole_from = first_of(last_row / group);
+            const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
+            const uint32_t s_at = lanes + half * G::kS, w_at = s_at + G::kW, o_at = lanes + G::kO + half * D;
+            float m = -INFINITY, l = 0.0f;
+            for (int j = 0; j < tiles; ++j) {
+                mbar_wait(&bar->s_full[half], j & 1, dead, limit);
+                dead = __any_sync(0xffffffffu, dead);
+                if (dead) break;
+                tc_fence_after();
+                // The last tile's scores of these positions are there: so are all products issued before them, and the operand tiles that they read
+                // are free. (Each commit of its own costs the tensor cores several hundred cycles.)
+                if (int(half) == halves_used - 1 && (tid & 127) == 0) {
+                    mbar_arrive(&bar->k_free[j & 1]);
+                    if (j > 0) mbar_arrive(&bar->v_free[(j - 1) & 1]);
+                }
+                const int base = begin + j * kN;
+                const bool whole = base + kN - 1 <= whole_to && base >= whole_from;
+                // tensor memory gives a warp little more than 32 bytes a cycle: the scores are read once and stay in registers
+                uint32_t x[kN / 32][32];
+#pragma unroll
+                for (int ch = 0; ch < kN / 32; ++ch) tmem_ld32(s_at + ch * 32, x[ch]);
+                tmem_wait_ld();
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) {
+                        if (base + i > last || base + i < first) x[i / 32][i % 32] = 0xff800000u;  // -inf
+                    }
+                }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < kN; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(__uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1])));
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
+                // the maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do
+                const bool above = top > m + 8.0f;
+                if (__any_sync(0xffffffffu, above)) {
+                    const float next = above ? top : m, keep = m == next ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - next);
+                    m = next;
+                    l *= keep;
+                    if (j != 0) {  // the product before this tile's scores is complete, as they are
+#pragma unroll
+                        for (int ch = 0; ch < D / 16; ++ch) {
+                            uint32_t y[16];
+                            tmem_ld16(o_at + ch * 16, y);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
+                            tmem_st16(o_at + ch * 16, y);
+                        }
+                    }
+                }
+                const float less = m == -INFINITY ? 0.0f : -m;
+                const f32x2 scale2 = pack2(scale, scale), less2 = pack2(less, less);
+                f32x2 sum[4] = {pack2(l, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+                auto weights = [&](auto all) {
+#pragma unroll
+                    for (int ch = 0; ch < kN / 32; ++ch) {
+                        uint32_t w[16], w_low[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const f32x2 v = fma2(pack2(x[ch][2 * i], x[ch][2 * i + 1]), scale2, less2);
+                            float y, z;
+                            if (decltype(all)::value && i % 4 < kByPolynomial) {
+                                exp2_by_polynomial(v, y, z);
+                            } else {
+                                unpack2(v, y, z);
+                                y = exp2_fast(y);
+                                z = exp2_fast(z);
+                            }
+                            sum[i & 3] = add2(sum[i & 3], pack2(y, z));
+                            const __half2 h = __floats2half2_rn(y, z);
+                            w[i] = bits(h);
+                            if (kTwo) w_low[i] = bits(__floats2half2_rn(y - __low2float(h), z - __high2float(h)));
+                        }
+                        tmem_st16(w_at + ch * 16, w);
+                        if (kTwo) tmem_st16(w_at + kN / 2 + ch * 16, w_low);
+                    }
+                };
+                if (whole && !kTwo) weights(std::true_type{});
+                else weights(std::false_type{});
+                float even, odd;
+                unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), even, odd);
+                l = even + odd;
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->p_full[half]);
+            }
+            if (!dead) mbar_wait(&bar->o_full, 0, dead, limit);
+            dead = __any_sync(0xffffffffu, dead);
+            tc_fence_after();
+            const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+            for (int ch = 0; ch < D / 32; ++ch) {
+                uint32_t x[32];
+                tmem_ld32(o_at + ch * 32, x);
+                tmem_wait_ld();
+                if (real) {
+                    if (a.wide) {
+                        constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+                        for (int i = 0; i < 32; i += kPer) {
+                            alignas(16) T y[kPer];
+#pragma unroll
+                            for (int u = 0; u < kPer; ++u) put(y + u, __uint_as_float(x[i + u]) * inverse);
+                            *reinterpret_cast<uint4*>(out + ch * 32 + i) = *reinterpret_cast<const uint4*>(y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) put(out + ch * 32 + i, __uint_as_float(x[i]) * inverse);
+                    }
+                }
+            }
+        } else if (real && tiles == 0) {  // rows that see nothing
+            for (int i = 0; i < D; ++i) put(out + i, 0.0f);
+        }
+    } else if (warp < 12) {
+        // ---- keys and values: 4 bits to f16 operand tiles ----
+        fewer_registers<96>();
+        const uint32_t p_tid = tid - 256;
+        // keys: lane = position, so that eight lanes write eight rows of the swizzled tile; a thread has kKeys blocks
+        constexpr int kBlocks = D / 32, kKeys = kN * kBlocks / 128;
+        const uint32_t block = (p_tid >> 5) % kBlocks, key_part = (p_tid >> 5) / kBlocks;
+        auto key_position = [&](int i) { return int((p_tid & 31) + 32 * (key_part + (4 / kBlocks) * i)); };
+        // values: a thread has 4 kWords bytes of 8 positions; eight lanes write eight chunks of one row
+        constexpr int kWords = D * kN >= 128 * 128 ? 2 : 1, kGroups = kN / 8, kPieces = D / 8 / kWords;
+        const uint32_t rest = p_tid >> 3, group8 = (p_tid & 7) + 8 * (rest % (kGroups / 8)), piece = rest / (kGroups / 8);
+        const bool has_values = piece < uint32_t(kPieces);
+        const uint32_t value_block = piece * kWords / 4;
+
+        auto page_at = [&](int p) { return p >= lo - int(c.page_size) && p <= hi && p >= 0 ? page_of(c, b, sequence, uint32_t(p) >> c.page_shift) : -1; };
+        uint4 key[kKeys];
+        __half key_scale[kKeys];
+        uint32_t value[8][kWords];
+        __half value_scale[8];
+        int key_page[kKeys], value_page;
+        auto ask_pages = [&](int j) {
+            const int base = begin + j * kN;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) key_page[i] = j < tiles ? page_at(base + key_position(i)) : -1;
+            value_page = j < tiles && has_values ? page_at(base + int(group8) * 8) : -1;
+        };
+        auto load_keys = [&](int j) {
+            const int base = begin + j * kN;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                const int p = base + key_position(i);
+                const bool there = key_page[i] >= 0 && p >= lo && p <= hi;
+                const size_t at = ((size_t(there ? key_page[i] : 0) * c.kv_heads + kv) * c.page_size + (uint32_t(p) & (c.page_size - 1))) * kBlocks + block;
+                key[i] = *reinterpret_cast<const uint4*>(c.k_quants + at * 16);
+                key_scale[i] = there ? c.k_scales[at] : __half(0.0f);
+            }
+        };
+        auto load_values = [&](int j) {
+            if (!has_values) return;
+            const int p = begin + j * kN + int(group8) * 8;
+            const size_t at = ((size_t(max(value_page, 0)) * c.kv_heads + kv) * c.page_size + (uint32_t(p) & (c.page_size - 1))) * kBlocks;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned char* src = c.v_quants + (at + i * kBlocks) * 16 + piece * kWords * 4;
+                if (kWords == 2) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(src);
+                    value[i][0] = x.x;
+                    value[i][kWords - 1] = x.y;
+                } else {
+                    value[i][0] = *reinterpret_cast<const uint32_t*>(src);
+                }
+                const bool there = value_page >= 0 && p + i >= lo && p + i <= hi;
+                value_scale[i] = there ? c.v_scales[at + i * kBlocks + value_block] : __half(0.0f);
+            }
+        };
+        ask_pages(0);
+        load_keys(0);
+        load_values(0);
+        ask_pages(1);
+        for (int j = 0; j < tiles; ++j) {
+            const uint32_t slot = j & 1;
+            if (j >= 2) mbar_wait(&bar->k_free[slot], (j >> 1) - 1 & 1, dead, limit);
+            dead = __any_sync(0xffffffffu, dead);
+            if (dead) break;
+            unsigned char* tile_k = smem + G::kKAt + slot * G::kK;
+#pragma unroll
+            for (int i = 0; i < kKeys; ++i) {
+                const uint32_t p = uint32_t(key_position(i)), w[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
+                const __half2 d = __half2half2(key_scale[i]);
+                unsigned char* row = tile_k + (block >> 1) * (kN * 128) + p * 128;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint32_t v[4];
+                    widen(w[u], d, v);
+                    *reinterpret_cast<uint4*>(row + ((((block & 1) * 4 + u) ^ (p & 7)) * 16)) = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->k_full[slot]);
+            if (j + 1 < tiles) load_keys(j + 1);
+
+            if (j >= 2) mbar_wait(&bar->v_free[slot], (j >> 1) - 1 & 1, dead, limit);
+            dead = __any_sync(0xffffffffu, dead);
+            if (dead) break;
+            unsigned char* tile_v = smem + G::kVAt + slot * G::kV;
+            if (has_values) {
+                __half2 d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = __halves2half2(value_scale[2 * i], value_scale[2 * i + 1]);
+                unsigned char* panel = tile_v + (group8 >> 3) * (D * 128);
+#pragma unroll
+                for (int x = 0; x < kWords; ++x) {
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {  // bytes 0, 1 and 2, 3 of the word
+                        uint32_t v[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) widen(__byte_perm(value[2 * i][x], value[2 * i + 1][x], z ? 0x7632 : 0x5410), d[i], v[i]);
+                        const uint32_t byte = (piece * kWords + x) * 4 + z * 2;  // of the row
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {  // (low, high) of the first byte, then of the second
+                            const uint32_t of = byte + (u >> 1), dim = (of >> 4) * 32 + (of & 15) + (u & 1) * 16;
+                            *reinterpret_cast<uint4*>(panel + dim * 128 + (((group8 & 7) ^ (dim & 7)) * 16)) = make_uint4(v[0][u], v[1][u], v[2][u], v[3][u]);
+                        }
+                    }
+                }
+            }
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar->v_full[slot]);
+            if (j + 1 < tiles) load_values(j + 1);
+            ask_pages(j + 2);
+        }
+    } else {
+        fewer_registers<32>();
+        if (warp == 12 && tiles != 0) {
+        // ---- products ----
+        constexpr uint32_t kScores = instr_f16(kN), kResult = instr_f16(D);
+        auto wait = [&](uint64_t* x, uint32_t parity) {
+            if (!dead) mbar_wait(x, parity, dead, limit);
+            dead = __any_sync(0xffffffffu, dead);
+            tc_fence_after();
+        };
+        auto scores = [&](int i, uint32_t slot) {  // S_i = Q_i K^T
+            if (elect_one()) {
+#pragma unroll
+                for (int part = 0; part < G::kParts; ++part) {
+#pragma unroll
+                    for (int s = 0; s < D / 16; ++s) {
+                        const uint32_t q = smem_at + (i * G::kParts + part) * G::kQ + (s >> 2) * G::kPanel + (s & 3) * 32;
+                        const uint32_t k = smem_at + G::kKAt + slot * G::kK + (s >> 2) * (kN * 128) + (s & 3) * 32;
+                        mma_ss(tmem + i * G::kS, smem_desc_swizzled(q), smem_desc_swizzled(k), kScores, part != 0 || s != 0);
+                    }
+                }
+                mma_commit(&bar->s_full[i]);
+            }
+            __syncwarp();
+        };
+        auto result = [&](int i, uint32_t slot, bool first) {  // O_i += P_i V
+            if (elect_one()) {
+#pragma unroll
+                for (int part = 0; part < G::kParts; ++part) {
+#pragma unroll
+                    for (int s = 0; s < kN / 16; ++s) {
+                        const uint32_t v = smem_at + G::kVAt + slot * G::kV + (s >> 2) * (D * 128) + (s & 3) * 32;
+                        mma_ts(tmem + G::kO + i * D, tmem + i * G::kS + G::kW + part * (kN / 2) + s * 8, smem_desc_swizzled(v), kResult, !(first && part == 0 && s == 0));
+                    }
+                }
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint64_t* x) {
+            if (elect_one()) mma_commit(x);
+            __syncwarp();
+        };
+        wait(&bar->k_full[0], 0);
+        for (int i = 0; i < halves_used && !dead; ++i) {
+            wait(&bar->q_full[i], 0);
+            if (!dead) scores(i, 0);
+        }
+        for (int j = 0; j < tiles && !dead; ++j) {
+            const uint32_t slot = j & 1, next = slot ^ 1;
+            wait(&bar->v_full[slot], j >> 1 & 1);
+            for (int i = 0; i < halves_used && !dead; ++i) {
+                wait(&bar->p_full[i], j & 1);
+                if (dead) break;
+                result(i, slot, j == 0);
+                if (j + 1 < tiles) {
+                    if (i == 0) wait(&bar->k_full[next], (j + 1) >> 1 & 1);
+                    if (dead) break;
+                    scores(i, next);  // over P_i: products run in the order in which they are issued
+                }
+            }
+        }
+        if (!dead) commit(&bar->o_full);
+        commit(&bar->drained);
+        mbar_drain(&bar->drained, 0);
+        }
+    }
+    release_next();
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+template <class T, int D>
+void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in, bool dependent, cudaStream_t s) {
+    const auto kernel = cache4_prompt_kernel<T, D>;
+    constexpr size_t smem = Prompt<D, sizeof(T) == 4>::kBytes;
+    static_assert(smem <= 227 * 1024);
+    static DeviceOnce once;
+    if (once.first()) BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    Cache4Attend a = in;
+    a.wide = (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (a.q_stride * sizeof(T)) | (a.out_stride * sizeof(T))) % 16 == 0;
+    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
+    uint32_t rows_per_cta = 256;
+    const uint64_t grid = (rows + rows_per_cta - 1) / rows_per_cta * c.kv_heads;
+    if (grid > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
+    if (dependent) {
+        launch_dependent(kernel, dim3(uint32_t(grid), b.sequences), dim3(kPromptThreads), smem, s, c, b, a, rows_per_cta);
+    } else {
+        kernel<<<dim3(uint32_t(grid), b.sequences), kPromptThreads, smem, s>>>(c, b, a, rows_per_cta);
+        BK_CUDA(cudaGetLastError());
+    }
+}
+
+}  // namespace
+
+bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a) {
+    return c.dim <= 128 && uint64_t(b.max_tokens) * (a.heads / c.kv_heads) > 64;
+}
+
+void launch_cache4_prompt(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s) {
+    if (c.dim == 64) {
+        if (type == T_F32) prompt_typed<float, 64>(c, b, a, dependent, s);
+        else if (type == T_F16) prompt_typed<__half, 64>(c, b, a, dependent, s);
+        else prompt_typed<__nv_bfloat16, 64>(c, b, a, dependent, s);
+    } else {
+        if (type == T_F32) prompt_typed<float, 128>(c, b, a, dependent, s);
+        else if (type == T_F16) prompt_typed<__half, 128>(c, b, a, dependent, s);
+        else prompt_typed<__nv_bfloat16, 128>(c, b, a, dependent, s);
+    }
+}
+
+}  // namespace bk
