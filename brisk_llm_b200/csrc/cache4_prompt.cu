@@ -115,8 +115,9 @@ template <int D, bool TWO> struct Prompt {
     static constexpr int kK = D / 64 * kN * 128, kV = kN / 64 * D * 128;
     static constexpr int kKAt = 2 * kParts * kQ, kVAt = kKAt + 2 * kK, kBarriersAt = kVAt + 2 * kV;
     static constexpr int kBytes = kBarriersAt + 256 + 1024;  // the tiles start on a 1024-byte boundary
-    // columns of tensor memory: a tile's scores, its weights (over the scores where they are one part), its result
-    static constexpr int kS = 128, kW = TWO ? 64 : 0, kO = 256;
+    // columns of tensor memory: the scores (which a tile of rows leaves at once for its registers, so one place does for both), each tile's
+    // weights and result
+    static constexpr int kW = 128, kO = 256;
 };
 constexpr int kByPolynomial = 1;  // of four pairs
 constexpr int kPromptThreads = 16 * 32;
@@ -124,7 +125,7 @@ template <int N> __device__ __forceinline__ void more_registers() { asm volatile
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 struct Bars {
-    uint64_t q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2], o_full, drained;
+    uint64_t q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], s_free, p_full[2], o_done[2], drained;
     uint32_t tmem;
 };
 
@@ -166,8 +167,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 mbar_init(&bar->v_free[i], 1);
                 mbar_init(&bar->s_full[i], 1);
                 mbar_init(&bar->p_full[i], 4);
+                mbar_init(&bar->o_done[i], 1);
             }
-            mbar_init(&bar->o_full, 1);
+            mbar_init(&bar->s_free, 4);
             mbar_init(&bar->drained, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
@@ -178,18 +180,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bar->tmem;
+    // All 512 columns are this CTA's, so they begin at 0: as a constant the address costs the products no move between registers.
+    constexpr uint32_t tmem = 0;
 
     auto last_of = [&](uint32_t token) { return int(max(min(context + token, held - 1), -1ll)); };
     auto first_of = [&](uint32_t token) { return a.window != 0 ? int(min(max(context + token - (long long)a.window + 1, 0ll), held)) : 0; };
     const int lo = first_of(row0 / group), hi = last_of((row0 + rows - 1) / group);
     const int begin = lo & ~(kN - 1), tiles = hi >= lo ? (hi - begin) / kN + 1 : 0, halves_used = rows > 128 ? 2 : 1;
     const long long limit = kTcWaitCycles;
-    bool dead = false;
+    bool dead = bar->tmem != 0;
 
     if (warp < 8) {
         // ---- softmax: a thread to a row ----
-        more_registers<192>();
+        more_registers<184>();
         const uint32_t half = warp >> 2, r = tid & 127, row = row0 + half * 128 + r;
         const bool real = half * 128 + r < rows;
         const uint32_t token = real ? row / group : 0, head = row - token * group;
@@ -231,19 +234,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             const uint32_t last_row = min(row0 + half * 128 + 127, row0 + rows - 1);
             const int whole_to = last_of((row0 + half * 128) / group), whole_from = first_of(last_row / group);
             const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
-            const uint32_t s_at = lanes + half * G::kS, w_at = s_at + G::kW, o_at = lanes + G::kO + half * D;
+            const uint32_t s_at = lanes, w_at = lanes + G::kW + half * 64, o_at = lanes + G::kO + half * D;
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < tiles; ++j) {
                 mbar_wait(&bar->s_full[half], j & 1, dead, limit);
                 dead = __any_sync(0xffffffffu, dead);
                 if (dead) break;
                 tc_fence_after();
-                // The last tile's scores of these positions are there: so are all products issued before them, and the operand tiles that they read
-                // are free. (Each commit of its own costs the tensor cores several hundred cycles.)
-                if (int(half) == halves_used - 1 && (tid & 127) == 0) {
-                    mbar_arrive(&bar->k_free[j & 1]);
-                    if (j > 0) mbar_arrive(&bar->v_free[(j - 1) & 1]);
-                }
+                // the last tile's scores: nobody reads these keys any more
+                if (int(half) == halves_used - 1 && (tid & 127) == 0) mbar_arrive(&bar->k_free[j & 1]);
                 const int base = begin + j * kN;
                 const bool whole = base + kN - 1 <= whole_to && base >= whole_from;
                 // tensor memory gives a warp little more than 32 bytes a cycle: the scores are read once and stay in registers
@@ -251,6 +250,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
 #pragma unroll
                 for (int ch = 0; ch < kN / 32; ++ch) tmem_ld32(s_at + ch * 32, x[ch]);
                 tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar->s_free);
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < kN; ++i) {
@@ -261,13 +263,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
 #pragma unroll
                 for (int i = 0; i < kN; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(__uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1])));
                 const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
+                if (j > 0) {  // the last weights have been read, the result is at rest
+                    mbar_wait(&bar->o_done[half], (j - 1) & 1, dead, limit);
+                    dead = __any_sync(0xffffffffu, dead);
+                    if (dead) break;
+                    tc_fence_after();
+                    if (int(half) == halves_used - 1 && (tid & 127) == 0) mbar_arrive(&bar->v_free[(j - 1) & 1]);
+                }
                 // the maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do
                 const bool above = top > m + 8.0f;
                 if (__any_sync(0xffffffffu, above)) {
                     const float next = above ? top : m, keep = m == next ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - next);
                     m = next;
                     l *= keep;
-                    if (j != 0) {  // the product before this tile's scores is complete, as they are
+                    if (j != 0) {
 #pragma unroll
                         for (int ch = 0; ch < D / 16; ++ch) {
                             uint32_t y[16];
@@ -316,7 +325,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->p_full[half]);
             }
-            if (!dead) mbar_wait(&bar->o_full, 0, dead, limit);
+            if (!dead) mbar_wait(&bar->o_done[half], (tiles - 1) & 1, dead, limit);
             dead = __any_sync(0xffffffffu, dead);
             tc_fence_after();
             const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
@@ -458,69 +467,74 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             ask_pages(j + 2);
         }
     } else {
-        fewer_registers<32>();
+        fewer_registers<48>();
         if (warp == 12 && tiles != 0) {
-        // ---- products ----
-        constexpr uint32_t kScores = instr_f16(kN), kResult = instr_f16(D);
-        auto wait = [&](uint64_t* x, uint32_t parity) {
-            if (!dead) mbar_wait(x, parity, dead, limit);
-            dead = __any_sync(0xffffffffu, dead);
-            tc_fence_after();
-        };
-        auto scores = [&](int i, uint32_t slot) {  // S_i = Q_i K^T
-            if (elect_one()) {
+            // ---- products ----
+            constexpr uint32_t kScores = instr_f16(kN), kResult = instr_f16(D);
+            const bool leader = elect_one();
+            // descriptors count in 16 bytes; what is added to them is a constant, or the slot's
+            const uint64_t q_desc = smem_desc_swizzled(smem_at), k_desc = smem_desc_swizzled(smem_at + G::kKAt), v_desc = smem_desc_swizzled(smem_at + G::kVAt);
+            auto wait = [&](uint64_t* x, uint32_t parity) {
+                if (!dead) mbar_wait(x, parity, dead, limit);
+                dead = __any_sync(0xffffffffu, dead);
+            };
+            auto scores = [&](auto half, uint64_t k) {  // S = Q_i K^T
+                constexpr int i = decltype(half)::value;
+                tc_fence_after();
+                if (leader) {
 #pragma unroll
-                for (int part = 0; part < G::kParts; ++part) {
+                    for (int part = 0; part < G::kParts; ++part) {
 #pragma unroll
-                    for (int s = 0; s < D / 16; ++s) {
-                        const uint32_t q = smem_at + (i * G::kParts + part) * G::kQ + (s >> 2) * G::kPanel + (s & 3) * 32;
-                        const uint32_t k = smem_at + G::kKAt + slot * G::kK + (s >> 2) * (kN * 128) + (s & 3) * 32;
-                        mma_ss(tmem + i * G::kS, smem_desc_swizzled(q), smem_desc_swizzled(k), kScores, part != 0 || s != 0);
+                        for (int s = 0; s < D / 16; ++s) {
+                            mma_ss(tmem, q_desc + ((i * G::kParts + part) * G::kQ + (s >> 2) * G::kPanel + (s & 3) * 32) / 16, k + ((s >> 2) * (kN * 128) + (s & 3) * 32) / 16, kScores,
+                                   part != 0 || s != 0);
+                        }
                     }
+                    mma_commit(&bar->s_full[i]);
                 }
-                mma_commit(&bar->s_full[i]);
-            }
-            __syncwarp();
-        };
-        auto result = [&](int i, uint32_t slot, bool first) {  // O_i += P_i V
-            if (elect_one()) {
+                __syncwarp();
+            };
+            auto result = [&](auto half, uint64_t v, bool first) {  // O_i += P_i V
+                constexpr int i = decltype(half)::value;
+                tc_fence_after();
+                if (leader) {
 #pragma unroll
-                for (int part = 0; part < G::kParts; ++part) {
+                    for (int part = 0; part < G::kParts; ++part) {
 #pragma unroll
-                    for (int s = 0; s < kN / 16; ++s) {
-                        const uint32_t v = smem_at + G::kVAt + slot * G::kV + (s >> 2) * (D * 128) + (s & 3) * 32;
-                        mma_ts(tmem + G::kO + i * D, tmem + i * G::kS + G::kW + part * (kN / 2) + s * 8, smem_desc_swizzled(v), kResult, !(first && part == 0 && s == 0));
+                        for (int s = 0; s < kN / 16; ++s) {
+                            mma_ts(tmem + G::kO + i * D, tmem + G::kW + i * 64 + part * (kN / 2) + s * 8, v + ((s >> 2) * (D * 128) + (s & 3) * 32) / 16, kResult, part != 0 || s != 0 || !first);
+                        }
                     }
+                    mma_commit(&bar->o_done[i]);
                 }
-            }
-            __syncwarp();
-        };
-        auto commit = [&](uint64_t* x) {
-            if (elect_one()) mma_commit(x);
-            __syncwarp();
-        };
-        wait(&bar->k_full[0], 0);
-        for (int i = 0; i < halves_used && !dead; ++i) {
-            wait(&bar->q_full[i], 0);
-            if (!dead) scores(i, 0);
-        }
-        for (int j = 0; j < tiles && !dead; ++j) {
-            const uint32_t slot = j & 1, next = slot ^ 1;
-            wait(&bar->v_full[slot], j >> 1 & 1);
-            for (int i = 0; i < halves_used && !dead; ++i) {
-                wait(&bar->p_full[i], j & 1);
-                if (dead) break;
-                result(i, slot, j == 0);
-                if (j + 1 < tiles) {
-                    if (i == 0) wait(&bar->k_full[next], (j + 1) >> 1 & 1);
-                    if (dead) break;
-                    scores(i, next);  // over P_i: products run in the order in which they are issued
+                __syncwarp();
+            };
+            // scores of tile j, then the product of the weights of tile j - 1: a tile's softmax has the products of the other for its time
+            uint32_t turns = 0;
+            auto turn = [&](auto half, int j) {
+                constexpr int i = decltype(half)::value;
+                if (j < tiles) {
+                    if (i == 0) wait(&bar->k_full[j & 1], j >> 1 & 1);
+                    if (j == 0) wait(&bar->q_full[i], 0);
+                    if (turns != 0) wait(&bar->s_free, (turns - 1) & 1);
+                    if (dead) return;
+                    scores(half, k_desc + (j & 1) * (G::kK / 16));
+                    ++turns;
                 }
+                if (j > 0) {
+                    if (i == 0) wait(&bar->v_full[(j - 1) & 1], (j - 1) >> 1 & 1);
+                    wait(&bar->p_full[i], (j - 1) & 1);
+                    if (dead) return;
+                    result(half, v_desc + ((j - 1) & 1) * (G::kV / 16), j == 1);
+                }
+            };
+            for (int j = 0; j <= tiles && !dead; ++j) {
+                turn(std::integral_constant<int, 0>{}, j);
+                if (halves_used == 2 && !dead) turn(std::integral_constant<int, 1>{}, j);
             }
-        }
-        if (!dead) commit(&bar->o_full);
-        commit(&bar->drained);
-        mbar_drain(&bar->drained, 0);
+            if (leader) mma_commit(&bar->drained);
+            __syncwarp();
+            mbar_drain(&bar->drained, 0);
         }
     }
     release_next();
