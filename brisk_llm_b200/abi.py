@@ -17,7 +17,7 @@ ARCH_BY_NAME = {"qwen3": ARCH_QWEN3, "llama": ARCH_LLAMA, "bitnet": ARCH_BITNET,
                 "smollm3": ARCH_LLAMA,
                 "qwen2": ARCH_QWEN3,
                 "phi3": ARCH_QWEN3}  # Phi-3/4-mini: NeoX rotation of the first rope_dim values, no Q/K norms  # Qwen2/2.5: the Qwen3 layer without Q/K norms, with q/k/v biases  # llama-shaped; its layers without RoPE are flagged per layer
-FLAG_NO_GRAPH, FLAG_NO_MEGAKERNEL, FLAG_NO_PERSISTENT = 1, 2, 4
+FLAG_NO_GRAPH, FLAG_NO_MEGAKERNEL, FLAG_NO_PERSISTENT, FLAG_CACHE_4BIT = 1, 2, 4, 8
 
 
 class Matrix(C.Structure):

@@ -547,6 +547,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     }
 }
 
+uint32_t multiprocessors() {
+    int dev = 0, count = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+    return uint32_t(count);
+}
+
 template <class T, int D>
 void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in, bool dependent, cudaStream_t s) {
     const auto kernel = cache4_prompt_kernel<T, D>;
@@ -557,7 +563,10 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
     Cache4Attend a = in;
     a.wide = (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (a.q_stride * sizeof(T)) | (a.out_stride * sizeof(T))) % 16 == 0;
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
-    uint32_t rows_per_cta = 256;
+    // Two tiles of rows share their keys and values where there are CTAs for all SMs all the same. us with 128 / 256 rows a CTA, bf16 heads
+    // of 128: 512 tokens of 32 heads (128 or 64 CTAs) 17 / 20, 3000 positions further on 68 / 79; 16 sequences of 64 tokens after 1000 (256
+    // or 128) 56 / 37.
+    const uint32_t rows_per_cta = (rows + 127) / 128 * c.kv_heads * b.sequences > multiprocessors() ? 256 : 128;
     const uint64_t grid = (rows + rows_per_cta - 1) / rows_per_cta * c.kv_heads;
     if (grid > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
     if (dependent) {
@@ -570,8 +579,13 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
 
 }  // namespace
 
+// A CTA of this kernel takes its positions one after another, about 2 us for 128 of them and up to 128 rows; the kernel of few rows takes 32 rows
+// at a time and spreads their positions. So this one needs rows enough for that to cost the other more: per sequence and
+// key/value head over 32, and 160 times 32 rows in all. us of few / many rows, bf16 heads of 128 after 2000 to 4000 positions: 128 x 32 rows 54 / 76
+// and 32 / 41, 192 x 32 61 / 42, 256 x 32 86 / 67, 512 x 32 167 / 68; f32 43 / 50, 79 / 95, 84 / 53, 127 / 83.
 bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a) {
-    return c.dim <= 128 && uint64_t(b.max_tokens) * (a.heads / c.kv_heads) > 64;
+    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
+    return c.dim <= 128 && rows > 32 && (rows + 31) / 32 * c.kv_heads * b.sequences >= 160;
 }
 
 void launch_cache4_prompt(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s) {

@@ -15,6 +15,7 @@
 
 #include "../../include/brisk_cuda.h"
 #include "attn_decode.h"
+#include "cache4.h"
 #include "kernels.h"
 
 namespace bk {
@@ -65,6 +66,16 @@ namespace {
 
 constexpr uint32_t kMaxBatch = 512;   // tokens per prefill pass (the reference: 256 on the CPU, 512 on Metal)
 constexpr uint32_t kMaxScored = 64;   // Engine::kMaxScoredTokens, src/engine.h:32
+constexpr uint32_t kCache4Page = 64;  // positions of a page of a 4-bit cache; a session's pages lie one after another
+
+// Bytes of one layer's keys or values in 4 bits: numbers and scales of whole pages.
+struct Cache4Bytes {
+    uint64_t pages, quants, scales;
+    Cache4Bytes(uint64_t context, uint64_t kv_heads, uint64_t dim) : pages((context + kCache4Page - 1) / kCache4Page) {
+        quants = pages * kCache4Page * kv_heads * (dim / 2);
+        scales = pages * kCache4Page * kv_heads * (dim / 16);
+    }
+};
 
 }  // namespace
 
@@ -92,6 +103,7 @@ struct Layer {
     bool slides = false;                                                  // Gemma: sliding-window layer with the local RoPE table
     bool no_rope = false;                                                 // SmolLM3: the layer attends without rotation
     __half *k_cache = nullptr, *v_cache = nullptr;
+    Cache4 cache4;  // instead of the two, in a session whose cache is held in 4 bits
 };
 
 std::string gb(uint64_t bytes) {
@@ -119,17 +131,22 @@ brisk_cuda_memory estimate(const brisk_cuda_model& m, const brisk_cuda_options& 
         e.weights += (2 * hidden + (L.q_norm ? dim : 0) + (L.k_norm ? dim : 0) + (L.attn_sub_norm ? q_dim : 0) + (L.ffn_sub_norm ? ffn : 0) +
                       (L.q_bias ? (q_dim + 2 * kv_dim) / tp : 0) + (L.attn_post_norm ? hidden : 0) + (L.ffn_post_norm ? hidden : 0)) * 4;
     }
+    const bool four_bits = (opt.flags & BRISK_CUDA_FLAG_CACHE_4BIT) != 0;
     e.cache = uint64_t(m.layer_count) * 2 * (kv_dim / tp) * ctx * 2;
+    if (four_bits) {
+        const Cache4Bytes c(ctx, m.kv_head_count / tp, dim);
+        e.cache = uint64_t(m.layer_count) * 2 * (c.quants + c.scales);
+    }
     const uint64_t widest = std::max(std::max(hidden, q_dim), ffn), batch = kMaxBatch;
     e.scratch += batch * (hidden + q_dim / tp + 2 * kv_dim / tp + q_dim / tp + 2 * ffn) * 4;  // residual, q, k, v, attended, gated, up
     e.scratch += batch * widest * (4 + 1 + 1) + batch * (widest / 32) * 8 + batch * (widest / 16) * 2 + batch * (widest / 256 + 1) * 4;  // activation planes
-    e.scratch += batch * (uint64_t(m.head_count) / tp) * ctx * 4;  // attention scores of one batch
+    if (!four_bits) e.scratch += batch * (uint64_t(m.head_count) / tp) * ctx * 4;  // attention scores of one batch
     e.scratch += uint64_t(kMaxScored) * vocab * 4;                 // logits
-    e.scratch += ctx * dim * 4 + (ctx + 1) * 4;                    // RoPE table, token history
-    if (m.sliding_window != 0) e.scratch += ctx * dim * 4;          // the sliding layers' RoPE table
+    e.scratch += (four_bits ? 2 * dim * 8 : ctx * dim * 4) + (ctx + 1) * 4;      // RoPE table (turns of the pairs), token history
+    if (m.sliding_window != 0 && !four_bits) e.scratch += ctx * dim * 4;  // the sliding layers' RoPE table
     if (m.gelu != 0 || m.final_softcap != 0.0f) e.scratch += tanh_table_bytes();  // corrections of the device's tanh
     for (uint32_t l = 0; l < m.layer_count; ++l) {
-        if (m.layers[l].no_rope) {
+        if (m.layers[l].no_rope && !four_bits) {
             e.scratch += ctx * dim * 4;  // the identity table of layers without rotation
             break;
         }
@@ -168,6 +185,8 @@ struct Session {
     int arch = 0, neox = 1, device = 0;
     uint32_t sms = 148;
     uint32_t flags = 0;
+    bool four_bits = false;  // BRISK_CUDA_FLAG_CACHE_4BIT: keys and values in 4 bits, attention of cache4_attn.cu and cache4_prompt.cu
+    float rope_attn_factor = 1.0f;
 
     // weights
     std::vector<std::unique_ptr<DevBuffer>> weight_buffers;
@@ -177,7 +196,7 @@ struct Session {
     uint64_t weight_bytes = 0, kv_bytes = 0;
 
     // state and scratch
-    DevBuffer kv, rope, rope_local, rope_none, proj_b, tanh_table, inputs_dev, hidden_b, q_b, k_b, v_b, attended_b, ffn_b, up_b, logits_b, tp_local, tp_gathered, full_b, actf, actq0, actd0, acts0, actqk,
+    DevBuffer kv, rope, rope_local, rope_none, turns, proj_b, tanh_table, inputs_dev, hidden_b, q_b, k_b, v_b, attended_b, ffn_b, up_b, logits_b, tp_local, tp_gathered, full_b, actf, actq0, actd0, acts0, actqk,
         actdk, actbs, partial, am_val, am_idx, history, logit_history, trace, topk_keys, topk_out, score_dev;
     DevActMut act;
     float* logits_host = nullptr;     // pinned [64][vocab]
@@ -352,6 +371,82 @@ struct Session {
         return out;
     }
 
+    // The f16 cache and the tables of its rotations.
+    void build_cache(const brisk_cuda_model& m) {
+        // K/V cache: per layer [kv head][max_context][head_dim] f16, K then V (src/model.cpp:982-991).
+        const size_t per = size_t(kv_heads_l) * max_context * head_dim;
+        kv_bytes = size_t(n_layers) * 2 * per * sizeof(__half);
+        kv.alloc(kv_bytes);
+        BK_CUDA(cudaMemsetAsync(kv.p, 0, kv_bytes, stream));
+        for (uint32_t l = 0; l < n_layers; ++l) {
+            layers[l].k_cache = kv.as<__half>() + size_t(l) * 2 * per;
+            layers[l].v_cache = layers[l].k_cache + per;
+        }
+
+        // RoPE table for every position, built like the reference builds it per batch (src/model.cpp:880-892):
+        // theta starts at the position and is multiplied by base^(-2/dim) per pair, in f32, with the host's libm.
+        // `width` values of a head rotate; the angles are built for that width (src/model.cpp:880-893). Rows keep the stride
+        // head_dim. cos and sin carry rope_attn_factor (:887-888).
+        const float attn_factor = rope_attn_factor;
+        auto build_rope = [&](DevBuffer& dst, float base, float scale, bool factors, uint32_t width) {
+            std::vector<float> table(size_t(max_context) * head_dim);
+            const float theta_scale = std::pow(base, -2.0f / static_cast<float>(width));
+            for (uint64_t p = 0; p < max_context; ++p) {
+                float theta = static_cast<float>(p) * scale;
+                float* r = table.data() + p * head_dim;
+                for (uint32_t i = 0; i < width / 2; ++i) {
+                    const float angle = factors && m.rope_factor_count != 0 ? theta / m.rope_factors[i] : theta;
+                    r[2 * i] = std::cos(angle) * attn_factor;
+                    r[2 * i + 1] = std::sin(angle) * attn_factor;
+                    theta *= theta_scale;
+                }
+            }
+            dst.alloc(table.size() * sizeof(float));
+            BK_CUDA(cudaMemcpy(dst.p, table.data(), table.size() * sizeof(float), cudaMemcpyHostToDevice));
+        };
+        build_rope(rope, rope_base, m.rope_scale != 0.0f ? m.rope_scale : 1.0f, true, rope_dim);
+        // The sliding layers rotate with their own base, an unscaled position and no per-frequency divisors (src/model.cpp:894).
+        if (sliding_window != 0) build_rope(rope_local, m.rope_base_local, 1.0f, false, head_dim);
+        // A layer without rotation (the reference rotates zero pairs there, src/model.cpp:1024) runs the same kernels over
+        // a table of cos = 1, sin = 0: x0 * 1 - x1 * 0 and x0 * 0 + x1 * 1 return x0 and x1 themselves.
+        if (unrotated_layers) {
+            std::vector<float> table(size_t(max_context) * head_dim);
+            for (size_t i = 0; i < table.size(); i += 2) {
+                table[i] = 1.0f;
+                table[i + 1] = 0.0f;
+            }
+            rope_none.alloc(table.size() * sizeof(float));
+            BK_CUDA(cudaMemcpy(rope_none.p, table.data(), table.size() * sizeof(float), cudaMemcpyHostToDevice));
+        }
+    }
+
+    // The cache in 4 bits: per layer the planes of cache4.h, all pages of the context one after another. Its kernels rotate by turns a
+    // position of each pair: [0, 128) those of the global layers, [128, 256) of the sliding ones (own base, unscaled, no divisors).
+    void build_cache4(const brisk_cuda_model& m) {
+        const Cache4Bytes per(max_context, kv_heads_l, head_dim);
+        kv_bytes = uint64_t(n_layers) * 2 * (per.quants + per.scales);
+        kv.alloc(kv_bytes);
+        BK_CUDA(cudaMemsetAsync(kv.p, 0, kv_bytes, stream));
+        for (uint32_t l = 0; l < n_layers; ++l) {
+            uint8_t* base = kv.as<uint8_t>() + uint64_t(l) * 2 * (per.quants + per.scales);  // every plane is a multiple of 256 bytes
+            Cache4& c = layers[l].cache4;
+            c.k_quants = base;
+            c.v_quants = base + per.quants;
+            c.k_scales = reinterpret_cast<__half*>(base + 2 * per.quants);
+            c.v_scales = reinterpret_cast<__half*>(base + 2 * per.quants + per.scales);
+            c.pages = uint32_t(per.pages); c.page_size = kCache4Page; c.kv_heads = kv_heads_l; c.dim = head_dim;
+            while ((1u << c.page_shift) < kCache4Page) ++c.page_shift;
+        }
+        std::vector<double> table(256);
+        char err[256];
+        if (brisk_cuda_rope_turns(rope_dim, rope_base, m.rope_scale != 0.0f ? m.rope_scale : 1.0f, m.rope_factor_count != 0 ? m.rope_factors : nullptr, table.data(), err, sizeof err) != 0 ||
+            (sliding_window != 0 && brisk_cuda_rope_turns(head_dim, m.rope_base_local, 1.0, nullptr, table.data() + 128, err, sizeof err) != 0)) {
+            throw CudaError(err);
+        }
+        turns.alloc(table.size() * sizeof(double));
+        BK_CUDA(cudaMemcpy(turns.p, table.data(), table.size() * sizeof(double), cudaMemcpyHostToDevice));
+    }
+
     void load(const brisk_cuda_model& m, const brisk_cuda_options& opt) {
         if (m.abi_version != BRISK_CUDA_ABI_VERSION) throw CudaError("cuda: model description has a different ABI version");
         tp_size = opt.tp_size > 1 ? opt.tp_size : 1;
@@ -360,6 +455,7 @@ struct Session {
         vocab = m.vocab_size; hidden = m.hidden; n_layers = m.layer_count; heads = m.head_count; kv_heads = m.kv_head_count;
         head_dim = m.head_dim; ffn = m.ffn; eps = m.rms_epsilon; rope_base = m.rope_base; arch = m.arch; neox = m.rope_neox;
         flags = opt.flags;
+        four_bits = (flags & BRISK_CUDA_FLAG_CACHE_4BIT) != 0;
         if (arch != BRISK_ARCH_QWEN3 && arch != BRISK_ARCH_LLAMA && arch != BRISK_ARCH_BITNET && arch != BRISK_ARCH_GEMMA3) {
             throw CudaError("cuda: unknown architecture id in the model description");
         }
@@ -468,51 +564,9 @@ struct Session {
             // A tied head is streamed once per token as the head; the embedding lookup reads one row of it.
         }
 
-        // K/V cache: per layer [kv head][max_context][head_dim] f16, K then V (src/model.cpp:982-991).
-        const size_t per = size_t(kv_heads_l) * max_context * head_dim;
-        kv_bytes = size_t(n_layers) * 2 * per * sizeof(__half);
-        kv.alloc(kv_bytes);
-        BK_CUDA(cudaMemsetAsync(kv.p, 0, kv_bytes, stream));
-        for (uint32_t l = 0; l < n_layers; ++l) {
-            layers[l].k_cache = kv.as<__half>() + size_t(l) * 2 * per;
-            layers[l].v_cache = layers[l].k_cache + per;
-        }
-
-        // RoPE table for every position, built like the reference builds it per batch (src/model.cpp:880-892):
-        // theta starts at the position and is multiplied by base^(-2/dim) per pair, in f32, with the host's libm.
-        // `width` values of a head rotate; the angles are built for that width (src/model.cpp:880-893). Rows keep the stride
-        // head_dim. cos and sin carry rope_attn_factor (:887-888).
-        const float attn_factor = m.rope_attn_factor != 0.0f ? m.rope_attn_factor : 1.0f;
-        auto build_rope = [&](DevBuffer& dst, float base, float scale, bool factors, uint32_t width) {
-            std::vector<float> table(size_t(max_context) * head_dim);
-            const float theta_scale = std::pow(base, -2.0f / static_cast<float>(width));
-            for (uint64_t p = 0; p < max_context; ++p) {
-                float theta = static_cast<float>(p) * scale;
-                float* r = table.data() + p * head_dim;
-                for (uint32_t i = 0; i < width / 2; ++i) {
-                    const float angle = factors && m.rope_factor_count != 0 ? theta / m.rope_factors[i] : theta;
-                    r[2 * i] = std::cos(angle) * attn_factor;
-                    r[2 * i + 1] = std::sin(angle) * attn_factor;
-                    theta *= theta_scale;
-                }
-            }
-            dst.alloc(table.size() * sizeof(float));
-            BK_CUDA(cudaMemcpy(dst.p, table.data(), table.size() * sizeof(float), cudaMemcpyHostToDevice));
-        };
-        build_rope(rope, rope_base, m.rope_scale != 0.0f ? m.rope_scale : 1.0f, true, rope_dim);
-        // The sliding layers rotate with their own base, an unscaled position and no per-frequency divisors (src/model.cpp:894).
-        if (sliding_window != 0) build_rope(rope_local, m.rope_base_local, 1.0f, false, head_dim);
-        // A layer without rotation (the reference rotates zero pairs there, src/model.cpp:1024) runs the same kernels over
-        // a table of cos = 1, sin = 0: x0 * 1 - x1 * 0 and x0 * 0 + x1 * 1 return x0 and x1 themselves.
-        if (unrotated_layers) {
-            std::vector<float> table(size_t(max_context) * head_dim);
-            for (size_t i = 0; i < table.size(); i += 2) {
-                table[i] = 1.0f;
-                table[i + 1] = 0.0f;
-            }
-            rope_none.alloc(table.size() * sizeof(float));
-            BK_CUDA(cudaMemcpy(rope_none.p, table.data(), table.size() * sizeof(float), cudaMemcpyHostToDevice));
-        }
+        rope_attn_factor = m.rope_attn_factor != 0.0f ? m.rope_attn_factor : 1.0f;
+        if (four_bits) build_cache4(m);
+        else build_cache(m);
 
         const uint32_t widest = std::max(std::max(hidden, q_dim), ffn);
         inputs_dev.alloc((kInputTokens + kMaxBatch + 4) * sizeof(int32_t));
@@ -544,7 +598,7 @@ struct Session {
         actbs.alloc(size_t(kMaxBatch) * (widest / 16) * 2);
         act.f32 = actf.as<float>(); act.q0 = actq0.as<int8_t>(); act.d0 = actd0.as<float>(); act.s0 = acts0.as<int32_t>();
         act.qk = actqk.as<int8_t>(); act.dk = actdk.as<float>(); act.bs = actbs.as<int16_t>();
-        partial.alloc(attn_scratch_floats(kMaxBatch, heads_l, uint32_t(max_context)) * 4);
+        if (!four_bits) partial.alloc(attn_scratch_floats(kMaxBatch, heads_l, uint32_t(max_context)) * 4);
         if (tp_size > 1) {
             const size_t widest_rows = std::max<size_t>(std::max<size_t>(q_dim, ffn), std::max<size_t>(hidden, size_t(vocab) * kMaxScored / kMaxBatch + 1));
             tp_local.alloc(size_t(kMaxBatch) * widest_rows / tp * 4 + 256);
@@ -577,7 +631,8 @@ struct Session {
 
     void plan_step() {
         const char* env = std::getenv("BRISK_CUDA_STEP");
-        if (tp_size > 1) step_note = "off: tensor parallel steps exchange activations between the operations";
+        if (four_bits) step_note = "off: over a cache in 4 bits single tokens take one kernel per operation";
+        else if (tp_size > 1) step_note = "off: tensor parallel steps exchange activations between the operations";
         else if (unrotated_layers) step_note = "off: layers without RoPE take the per-operation kernels (the persistent kernel rotates every layer with one table)";
         else if (variant_layers) step_note = "off: Gemma layer variants (post-norms, GELU, sliding window), 256-wide heads and partial rotary take one kernel per operation";
         else if (flags & (BRISK_CUDA_FLAG_NO_MEGAKERNEL | BRISK_CUDA_FLAG_NO_PERSISTENT)) step_note = "off: disabled by the session's flags";
@@ -767,6 +822,7 @@ struct Session {
     // Whether single tokens take the fused kernels: partial rotary does not, and what only the kernels of attn_decode.cu cover
     // (windows, 256-wide heads) needs a context that fits them.
     bool single_kernels() const {
+        if (four_bits) return true;  // its attention takes whatever the layers are
         if (!variant_layers) return true;
         return rope_dim == head_dim && attn_decode_runs();
     }
@@ -861,11 +917,13 @@ struct Session {
             // 2064 positions of the 0.6B shape Q4_0 up to 7 % slower, Q8_0 1 % faster), from 6.6 M on either way with the tokens: 2560 x
             // 2560 at 17 and 23 1159/1262, 1295/1274, 4096 x 4096 2286/2210, 2186/2236.
             const bool planes = !single && !tp && L.attn_sub_norm == nullptr && block_elems(L.o.type) == 32 &&
-                uint64_t(hidden) * q_dim <= (n <= 16 ? kPlanesOneTile : kPlanesTwoTiles) && attention_takes_chain(n);
+                uint64_t(hidden) * q_dim <= (n <= 16 ? kPlanesOneTile : kPlanesTwoTiles) && attention_takes_chain(n) && !four_bits;
             const DevActMut* attended_planes = planes ? &act : nullptr;
             {
                 Scope sc(this, PH_ATTENTION);
-                if (single) {
+                if (four_bits) {
+                    attend4(L, n, max_visible);
+                } else if (single) {
                     launches += launch_dec_attention(r, at, fused_attention, sms, stream);
                 } else {
                     launch_qk_norm_rope_store(r, stream);
@@ -971,6 +1029,26 @@ struct Session {
         soft_cap(1);
     }
 
+    // Norm and rotation of the batch's queries and keys, keys and values into the 4-bit cache, attention over it.
+    void attend4(const Layer& L, uint32_t n, uint32_t max_visible) {
+        Cache4Batch b;
+        b.context = reinterpret_cast<const int32_t*>(d_position());
+        b.sequences = 1; b.columns = L.cache4.pages; b.tokens = b.max_tokens = n; b.max_length = max_visible;
+        Cache4Append a;
+        a.q = a.q_out = q_b.p; a.k = k_b.p; a.v = v_b.p;
+        a.q_stride = a.q_out_stride = q_dim_l; a.k_stride = a.v_stride = kv_dim_l;
+        a.q_norm = L.q_norm; a.k_norm = L.k_norm; a.q_bias = L.q_bias; a.k_bias = L.k_bias; a.v_bias = L.v_bias;
+        a.turns = turns.as<double>() + (L.slides ? 128 : 0);
+        a.heads = heads_l; a.rope_dim = L.no_rope ? 0 : L.slides ? head_dim : rope_dim; a.adjacent = !neox;
+        a.eps = eps; a.attn_factor = rope_attn_factor;
+        launch_cache4_append(L.cache4, b, a, T_F32, true, stream);
+        Cache4Attend at;
+        at.q = q_b.p; at.out = attended_b.p; at.q_stride = at.out_stride = q_dim_l;
+        at.heads = heads_l; at.window = L.slides ? sliding_window : 0; at.scale = 1.0f / std::sqrt(static_cast<float>(head_dim));
+        launch_cache4_attention(L.cache4, b, at, T_F32, true, stream);
+        launches += 2;
+    }
+
     // Output norm and head of rows [first, first + rows) of the residual stream, at most kMaxScored of them, into logits_b.
     void head_rows(uint32_t first, uint32_t rows) {
         Needs nd;
@@ -1003,7 +1081,7 @@ struct Session {
     bool token_active() const { return token_enabled && !profiling; }
     void forward_decode(bool persistent) {
         if (!persistent) {
-            run_layers(1, LAST_LOGITS, uint32_t(max_context), true);
+            run_layers(1, LAST_LOGITS, step_bound(), true);
             return;
         }
         if (token_enabled) {
@@ -1088,7 +1166,12 @@ struct Session {
     // Up to 512 visible positions the attention of a single token is one kernel (attn_decode.cu; its K rows are requested ahead
     // of the projections: 0.6B shape, one kernel per operation, at 181 positions 719 -> 661 us a token, at 520 - a second, late
     // round of rows - 757 -> 790).
+    // Over a 4-bit cache it is the same kernel in both forms, which shares the positions among more CTAs where there may be many (one token of 8
+    // key/value heads at 517 positions: 6.5 us with 4 CTAs a head, 7.5 with 16).
+    static constexpr uint32_t kShort4 = 512;
+    uint32_t step_bound() const { return uint32_t(four_bits && fused_attention ? std::min<uint64_t>(kShort4, max_context) : max_context); }  // of a replayed step
     bool takes_fused_attention(uint64_t visible) const {
+        if (four_bits) return visible <= kShort4;
         return visible <= 512 && head_dim <= 128 && rope_dim == head_dim && attn_decode_runs();
     }
     // One kernel per operation also beats the persistent kernel, at every depth and position. Persistent / per operation, us a token
@@ -1122,10 +1205,10 @@ struct Session {
         if (!single_kernels()) batched = true;
         // The fused weighted sum keeps a head's probabilities of the whole context in shared memory; past that the batched
         // kernels, which have no such limit, take single tokens too.
-        const bool too_long = !persistent && !variant_layers &&
+        const bool too_long = !persistent && !variant_layers && !four_bits &&
                               !dec_attention_fits(uint32_t(max_context), heads_l, head_dim, sms);
         if ((flags & BRISK_CUDA_FLAG_NO_MEGAKERNEL) || too_long) {
-            forward(1, LAST_LOGITS, uint32_t(max_context));  // the batched kernels, one token
+            forward(1, LAST_LOGITS, step_bound());  // the batched kernels, one token
             return;
         }
         if (persistent) ++persistent_steps;

@@ -145,6 +145,9 @@ typedef struct brisk_cuda_options {
 #define BRISK_CUDA_FLAG_NO_MEGAKERNEL 2u /* single-token steps through the batched kernels instead of the fused ones */
 #define BRISK_CUDA_FLAG_NO_PERSISTENT 4u /* single-token steps as one fused kernel per operation (replayed as a CUDA graph)
                                             instead of one persistent kernel for all layers */
+#define BRISK_CUDA_FLAG_CACHE_4BIT 8u    /* keys and values held in 4 bits (28 % of the f16 bytes) as brisk_cuda_cache4_append stores them, attention as
+                                            brisk_cuda_cache4_attention computes it: no longer the reference's bits, results as far from them as
+                                            16 steps for every 32 values put them. Contexts and models as with the f16 cache */
 
 typedef struct brisk_cuda_session brisk_cuda_session;
 
@@ -266,7 +269,7 @@ int brisk_cuda_argmax_static(const float* logits, uint32_t vocab, uint32_t rows,
 /* ---- key/value cache in 4 bits, in pages ------------------------------------------------------------------------------
  * No counterpart in the reference (its cache is f16, contiguous, of one sequence). For embedders that keep the keys and values of
  * several sequences, or of long ones, in 28 % of the f16 bytes: rows are appended, attended to and read back by the three calls below.
- * All pointers are DEVICE pointers on the current device unless
+ * Sessions created with BRISK_CUDA_FLAG_CACHE_4BIT run their layers over them. All pointers are DEVICE pointers on the current device unless
  * they are said to be host ones; `stream` is a cudaStream_t (NULL: the default stream). The calls launch on the stream and return: no
  * allocation, no synchronisation, no workspace, nothing kept - they may be captured into a graph and replayed, with context,
  * page_table and query_start read at every replay. They return 0, or -1 and a message in err before anything is launched.

@@ -232,6 +232,10 @@ ATTENDS = [
     (8, 2, 128, [1500, 0, 700], [333, 257, 1], 64, 400),
     (32, 4, 64, [255], [520], 128, 0),
     (4, 4, 128, [9000], [1], 64, 0),
+    # rows enough for the kernel of many, and for two tiles of them to a CTA
+    (21, 3, 64, [100], [300], 16, 0),
+    (32, 8, 128, [0, 100, 5], [256, 200, 301], 32, 0),
+    (56, 8, 64, [31, 0], [290, 150], 64, 70),
 ]
 
 
@@ -244,7 +248,7 @@ def test_attention_is_the_definition_s(case, type):
 
 
 @pytest.mark.parametrize("type", ["f32", "bf16"])
-@pytest.mark.parametrize("tokens", [1, 40, 300])
+@pytest.mark.parametrize("tokens", [1, 40, 300, 700])
 def test_attention_of_large_scores(type, tokens):
     """Scores of some hundreds: one position has all the weight, and the running maximum moves often."""
     w = World(4, 2, 128, [500], [tokens])
@@ -256,7 +260,7 @@ def test_even_batches_without_a_table():
     check_attention(w, 8, "f32")
 
 
-@pytest.mark.parametrize("tokens", [1, 200])
+@pytest.mark.parametrize("tokens", [1, 200, 1300])
 def test_a_sequence_that_sees_nothing_and_pages_outside_the_pool(tokens):
     import torch
     w = World(6, 2, 64, [100, 40], [tokens, tokens])
@@ -296,11 +300,12 @@ def test_a_sequence_that_sees_nothing_and_pages_outside_the_pool(tokens):
     assert (got[:tokens] == 0).all() and torch.isfinite(got).all()
 
 
-def test_positions_past_the_columns_are_not_seen():
+@pytest.mark.parametrize("heads", [2, 128])
+def test_positions_past_the_columns_are_not_seen(heads):
     import torch
     w = World(7, 1, 128, [60], [40], spare_columns=0)  # two columns hold 128 positions
     w.batch.context.copy_(w.dev(np.array([100], np.int32)))  # ... and 12 of the 40 tokens stand past them
-    q = torch.randn((40, 2, 128), device=w.device)
+    q = torch.randn((40, heads, 128), device=w.device)
     planes = w.planes()
     got = w.cache.attention(w.batch, q).cpu().numpy()
     k, v = w.values(0, 128)
@@ -315,7 +320,7 @@ def test_positions_past_the_columns_are_not_seen():
     assert np.array_equal(after[0].transpose(0, 2, 1, 3)[~touched], planes[0].transpose(0, 2, 1, 3)[~touched])
 
 
-@pytest.mark.parametrize("tokens", [1, 3, 150])
+@pytest.mark.parametrize("tokens", [1, 3, 150, 400])
 def test_bounds_that_are_not_given_change_nothing(tokens):
     import torch
     from brisk_llm_b200 import cache4
@@ -353,7 +358,7 @@ def test_a_prompt_at_once_and_token_by_token():
     assert (a - torch.cat(b)).abs().max() <= 2e-5 * a.abs().max()
 
 
-@pytest.mark.parametrize("tokens", [1, 140])
+@pytest.mark.parametrize("tokens", [1, 140, 320])
 def test_captured_and_replayed_on_two_streams(tokens):
     """A captured append and attention, replayed for other positions and pages; two graphs at a time on two streams."""
     import torch
