@@ -410,14 +410,12 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
             }
         }
 
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            // the positions of this lane's two pairs (see position_of); what the tile's rows do not see has scale 0, whatever lies there
-            const uint32_t pos[4] = {16 * h + t, 16 * h + 4 + (t ^ (D == 128 ? 1 : 2)), 16 * h + 8 + t, 16 * h + 12 + (t ^ (D == 128 ? 1 : 2))};
-            constexpr int kWords = D / 64;
-            uint32_t w[4][kWords];
+        constexpr int kWords = D / 64;
+        const uint32_t value_block = D == 64 ? g >> 2 : D == 128 ? g >> 1 : g;
+        // Values of 16 positions as this lane's two pairs (see position_of); what the tile's rows do not see has scale 0, whatever lies there.
+        auto load_values = [&](int h, uint32_t (&w)[4][kWords], __half2 (&pair)[2]) {
+            const uint32_t odd = t ^ (D == 128 ? 1 : 2), pos[4] = {16 * h + t, 16 * h + 4 + odd, 16 * h + 8 + t, 16 * h + 12 + odd};
             __half d[4];
-            const uint32_t block = D == 64 ? g >> 2 : D == 128 ? g >> 1 : g;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const unsigned char* row = st + G::kV + pos[i] * G::kRow;
@@ -430,7 +428,7 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                     const uint4 x = *reinterpret_cast<const uint4*>(row + chunk_of<D>(pos[i], g) * 16);
                     w[i][0] = x.x; w[i][1 % kWords] = x.y; w[i][2 % kWords] = x.z; w[i][kWords - 1] = x.w;
                 }
-                d[i] = *reinterpret_cast<const __half*>(st + G::kVs + pos[i] * G::kScales + block * 2);
+                d[i] = *reinterpret_cast<const __half*>(st + G::kVs + pos[i] * G::kScales + value_block * 2);
             }
             if (!whole) {
 #pragma unroll
@@ -439,21 +437,59 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                     if (p < lo || p > hi) d[i] = __half(0.0f);
                 }
             }
-            const __half2 d0 = __halves2half2(d[0], d[1]), d1 = __halves2half2(d[2], d[3]);
+            pair[0] = __halves2half2(d[0], d[1]);
+            pair[1] = __halves2half2(d[2], d[3]);
+        };
+        if constexpr (kTwo) {
+            // A product cuts its sum off at 24 bits: adding to a long sum each time loses a third of a bit of it per product, all one way. The tile's
+            // products make a sum of their own, and that is added with rounding.
+            uint32_t w[2][4][kWords];
+            __half2 pair[2][2];
+            load_values(0, w[0], pair[0]);
+            load_values(1, w[1], pair[1]);
 #pragma unroll
             for (int x = 0; x < kWords; ++x) {
 #pragma unroll
                 for (int z = 0; z < 2; ++z) {
-                    uint32_t v0[4], v1[4];
-                    widen(__byte_perm(w[0][x], w[1][x], z ? 0x7632 : 0x5410), d0, v0);
-                    widen(__byte_perm(w[2][x], w[3][x], z ? 0x7632 : 0x5410), d1, v1);
+                    uint32_t v[2][2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        widen(__byte_perm(w[h][0][x], w[h][1][x], z ? 0x7632 : 0x5410), pair[h][0], v[h][0]);
+                        widen(__byte_perm(w[h][2][x], w[h][3][x], z ? 0x7632 : 0x5410), pair[h][1], v[h][1]);
+                    }
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int i = x * 4 + z * 2 + u;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            mma16816(o[i][n], v0[2 * u], v0[2 * u + 1], v1[2 * u], v1[2 * u + 1], p_high[h][n][0], p_high[h][n][1]);
-                            if (kTwo) mma16816(o[i][n], v0[2 * u], v0[2 * u + 1], v1[2 * u], v1[2 * u + 1], p_low[h][n][0], p_low[h][n][1]);
+                            float y[4];
+                            mma16816(y, v[0][0][2 * u], v[0][0][2 * u + 1], v[0][1][2 * u], v[0][1][2 * u + 1], p_low[0][n][0], p_low[0][n][1], 0.0f, 0.0f);
+                            mma16816(y, v[1][0][2 * u], v[1][0][2 * u + 1], v[1][1][2 * u], v[1][1][2 * u + 1], p_low[1][n][0], p_low[1][n][1]);
+                            mma16816(y, v[0][0][2 * u], v[0][0][2 * u + 1], v[0][1][2 * u], v[0][1][2 * u + 1], p_high[0][n][0], p_high[0][n][1]);
+                            mma16816(y, v[1][0][2 * u], v[1][0][2 * u + 1], v[1][1][2 * u], v[1][1][2 * u + 1], p_high[1][n][0], p_high[1][n][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[i][n][e] += y[e];
+                        }
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[4][kWords];
+                __half2 pair[2];
+                load_values(h, w, pair);
+#pragma unroll
+                for (int x = 0; x < kWords; ++x) {
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        uint32_t v0[4], v1[4];
+                        widen(__byte_perm(w[0][x], w[1][x], z ? 0x7632 : 0x5410), pair[0], v0);
+                        widen(__byte_perm(w[2][x], w[3][x], z ? 0x7632 : 0x5410), pair[1], v1);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma16816(o[x * 4 + z * 2 + u][n], v0[2 * u], v0[2 * u + 1], v1[2 * u], v1[2 * u + 1], p_high[h][n][0], p_high[h][n][1]);
                         }
                     }
                 }

@@ -118,6 +118,9 @@ template <int D, bool TWO> struct Prompt {
     // columns of tensor memory: the scores (which a tile of rows leaves at once for its registers, so one place does for both), each tile's
     // weights and result
     static constexpr int kW = 128, kO = 256;
+    // A product cuts its sum off at 24 bits, a third of a bit lost each time, all one way: f32 results are added up over this many tiles only, and
+    // those sums with rounding, in the columns of the second tile of rows, which f32 does without.
+    static constexpr int kFlush = 4, kTotal = kO + D;
 };
 constexpr int kByPolynomial = 1;  // of four pairs
 constexpr int kPromptThreads = 16 * 32;
@@ -235,6 +238,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             const int whole_to = last_of((row0 + half * 128) / group), whole_from = first_of(last_row / group);
             const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
             const uint32_t s_at = lanes, w_at = lanes + G::kW + half * 64, o_at = lanes + G::kO + half * D;
+            auto scale_columns = [&](uint32_t at, float by) {
+#pragma unroll
+                for (int ch = 0; ch < D / 16; ++ch) {
+                    uint32_t y[16];
+                    tmem_ld16(at + ch * 16, y);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * by);
+                    tmem_st16(at + ch * 16, y);
+                }
+            };
+            auto add_up = [&](bool more) {  // the total is (or has added) the result of the last tiles
+#pragma unroll
+                for (int ch = 0; ch < D / 16; ++ch) {
+                    uint32_t y[16], z[16];
+                    tmem_ld16(o_at + ch * 16, y);
+                    if (more) tmem_ld16(lanes + G::kTotal + ch * 16, z);
+                    tmem_wait_ld();
+                    if (more) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) + __uint_as_float(z[i]));
+                    }
+                    tmem_st16(lanes + G::kTotal + ch * 16, y);
+                }
+                tmem_wait_st();
+            };
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < tiles; ++j) {
                 mbar_wait(&bar->s_full[half], j & 1, dead, limit);
@@ -269,6 +298,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     if (dead) break;
                     tc_fence_after();
                     if (int(half) == halves_used - 1 && (tid & 127) == 0) mbar_arrive(&bar->v_free[(j - 1) & 1]);
+                    if (kTwo && j % G::kFlush == 0) add_up(j > G::kFlush);
                 }
                 // the maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do
                 const bool above = top > m + 8.0f;
@@ -276,17 +306,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     const float next = above ? top : m, keep = m == next ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - next);
                     m = next;
                     l *= keep;
-                    if (j != 0) {
-#pragma unroll
-                        for (int ch = 0; ch < D / 16; ++ch) {
-                            uint32_t y[16];
-                            tmem_ld16(o_at + ch * 16, y);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * keep);
-                            tmem_st16(o_at + ch * 16, y);
-                        }
-                    }
+                    if (kTwo && j >= G::kFlush) scale_columns(lanes + G::kTotal, keep);
+                    if (kTwo ? j % G::kFlush != 0 : j != 0) scale_columns(o_at, keep);
                 }
                 const float less = m == -INFINITY ? 0.0f : -m;
                 const f32x2 scale2 = pack2(scale, scale), less2 = pack2(less, less);
@@ -334,6 +355,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 uint32_t x[32];
                 tmem_ld32(o_at + ch * 32, x);
                 tmem_wait_ld();
+                if (kTwo && tiles > G::kFlush) {
+                    uint32_t y[32];
+                    tmem_ld32(lanes + G::kTotal + ch * 32, y);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
+                }
                 if (real) {
                     if (a.wide) {
                         constexpr int kPer = 16 / sizeof(T);
@@ -483,11 +511,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 tc_fence_after();
                 if (leader) {
 #pragma unroll
-                    for (int part = 0; part < G::kParts; ++part) {
+                    for (int part = G::kParts - 1; part >= 0; --part) {  // the small parts first: a sum loses up to half a bit with every product
 #pragma unroll
                         for (int s = 0; s < D / 16; ++s) {
                             mma_ss(tmem, q_desc + ((i * G::kParts + part) * G::kQ + (s >> 2) * G::kPanel + (s & 3) * 32) / 16, k + ((s >> 2) * (kN * 128) + (s & 3) * 32) / 16, kScores,
-                                   part != 0 || s != 0);
+                                   part != G::kParts - 1 || s != 0);
                         }
                     }
                     mma_commit(&bar->s_full[i]);
@@ -525,7 +553,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     if (i == 0) wait(&bar->v_full[(j - 1) & 1], (j - 1) >> 1 & 1);
                     wait(&bar->p_full[i], (j - 1) & 1);
                     if (dead) return;
-                    result(half, v_desc + ((j - 1) & 1) * (G::kV / 16), j == 1);
+                    result(half, v_desc + ((j - 1) & 1) * (G::kV / 16), kTwo ? (j - 1) % G::kFlush == 0 : j == 1);
                 }
             };
             for (int j = 0; j <= tiles && !dead; ++j) {
@@ -566,7 +594,7 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
     // Two tiles of rows share their keys and values where there are CTAs for all SMs all the same. us with 128 / 256 rows a CTA, bf16 heads
     // of 128: 512 tokens of 32 heads (128 or 64 CTAs) 17 / 20, 3000 positions further on 68 / 79; 16 sequences of 64 tokens after 1000 (256
     // or 128) 56 / 37.
-    const uint32_t rows_per_cta = (rows + 127) / 128 * c.kv_heads * b.sequences > multiprocessors() ? 256 : 128;
+    const uint32_t rows_per_cta = sizeof(T) < 4 && (rows + 127) / 128 * c.kv_heads * b.sequences > multiprocessors() ? 256 : 128;
     const uint64_t grid = (rows + rows_per_cta - 1) / rows_per_cta * c.kv_heads;
     if (grid > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
     if (dependent) {
