@@ -13,6 +13,7 @@ read on the device when the work runs: a captured call that is replayed sees wha
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -20,6 +21,8 @@ from . import abi
 
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _ERR = 512
+_thread = threading.local()  # a buffer for messages, made once: a call's host part is a third of the shortest calls' time as it is
+_device, _stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _fail(message: str):
@@ -82,6 +85,7 @@ class Batch:
                 _fail(f"{name} must be from 0 to 2^31 - 1")
         s.sequences, s.table_columns, s.tokens, s.max_tokens, s.max_length = n, columns, tokens, max_tokens, max_length
         self.tokens = tokens
+        self.ref = C.byref(s)
 
 
 class PagedCache:
@@ -99,7 +103,7 @@ class PagedCache:
                 _fail(f"{name} must be a contiguous {dtype} tensor of shape {(pages, kv_heads, page_size, last)} on {self.device}")
         self.k_quants, self.k_scales, self.v_quants, self.v_scales = k_quants, k_scales, v_quants, v_scales
         self.c = abi.Cache4(k_quants.data_ptr(), k_scales.data_ptr(), v_quants.data_ptr(), v_scales.data_ptr(), pages, page_size, kv_heads, self.head_dim)
-        self._lib = abi.load_library()
+        self._lib, self._ref = abi.load_library(), C.byref(self.c)
 
     @classmethod
     def allocate(cls, pages: int, kv_heads: int, head_dim: int, page_size: int = 64, device="cuda"):
@@ -110,19 +114,18 @@ class PagedCache:
         return cls(plane(head_dim // 2, torch.uint8), plane(head_dim // 32, torch.float16), plane(head_dim // 2, torch.uint8),
                    plane(head_dim // 32, torch.float16))
 
-    def _rows(self, t, batch, heads, what, dtype=None):
-        """[tokens, heads, head_dim] with any stride between tokens; returns it."""
-        if t.dim() != 3 or t.shape[0] != batch.tokens or (heads and t.shape[1] != heads) or t.shape[2] != self.head_dim or t.device != self.device:
-            _fail(f"{what} must be [{batch.tokens}, {heads or 'heads'}, {self.head_dim}] on {self.device}")
-        if (dtype is not None and t.dtype != dtype) or t.dtype not in _TYPES:
-            _fail(f"{what} must be {dtype or 'float32, float16 or bfloat16'}")
-        if t.shape[0] and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != self.head_dim) or (t.shape[0] > 1 and t.stride(0) < t.shape[1] * self.head_dim)):
+    def _rows(self, t, tokens, heads, what, dtype):
+        """Checks [tokens, heads, head_dim] (heads 0: any number) with any stride between tokens; returns heads and that stride."""
+        shape, dim = t.shape, self.head_dim
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads and shape[1] != heads) or t.device != self.device:
+            _fail(f"{what} must be [{tokens}, {heads or 'heads'}, {dim}] on {self.device}")
+        if t.dtype != dtype:
+            _fail(f"{what} must be {dtype}")
+        heads = shape[1]
+        outer, middle, inner = t.stride()
+        if tokens and (inner != 1 or (middle != dim and heads > 1) or (outer < heads * dim and tokens > 1)):
             _fail(f"the heads of a token must lie side by side in {what}")
-        return t
-
-    @staticmethod
-    def _stride(t):
-        return max(t.stride(0), t.shape[1] * t.shape[2])  # of a single row any stride will do
+        return heads, max(outer, heads * dim)  # of a single row any stride will do
 
     def _vector(self, t, n, what):
         if t is None:
@@ -131,70 +134,78 @@ class PagedCache:
             _fail(f"{what} must be {n} contiguous float32 values on {self.device}")
         return t.data_ptr()
 
-    def _call(self, fn, *args):
-        err = C.create_string_buffer(_ERR)
-        index = self.device.index
-        if torch.cuda.current_device() == index:
-            rc = fn(self.c, *args, torch.cuda.current_stream(index).cuda_stream, err, _ERR)
-        else:
-            with torch.cuda.device(index):
-                rc = fn(self.c, *args, torch.cuda.current_stream(index).cuda_stream, err, _ERR)
-        if rc != 0:
-            raise RuntimeError(err.value.decode())
-
-    def _check(self, batch):
+    def _type(self, batch, t, what):
         if batch.device != self.device:
             _fail(f"the batch is on {batch.device}, the cache on {self.device}")
+        number = _TYPES.get(t.dtype)
+        if number is None:
+            _fail(f"{what} must be float32, float16 or bfloat16")
+        return number
+
+    def _call(self, fn, *args):
+        try:
+            err = _thread.err
+        except AttributeError:
+            err = _thread.err = C.create_string_buffer(_ERR)
+        index = self.device.index
+        if _device() == index:
+            rc = fn(self._ref, *args, _stream(index), err, _ERR)
+        else:
+            with torch.cuda.device(index):
+                rc = fn(self._ref, *args, _stream(index), err, _ERR)
+        if rc != 0:
+            raise RuntimeError(err.value.decode())
 
     def append(self, batch: Batch, q, k, v, rotary: Rotary | None = None, q_norm=None, k_norm=None, eps: float = 1e-6, q_bias=None, k_bias=None,
                v_bias=None, out=None):
         """Stores the batch's keys and values at their positions and returns its queries: biased, each head over its root mean square times
         its norm, rotated (the values only biased). q may be None: keys and values only. out may be q."""
-        self._check(batch)
-        dtype, kv, dim = k.dtype, self.kv_heads, self.head_dim
-        self._rows(k, batch, kv, "k")
-        self._rows(v, batch, kv, "v", dtype)
-        r = abi.Cache4Rows()
-        r.k, r.v, r.k_stride, r.v_stride = k.data_ptr(), v.data_ptr(), self._stride(k), self._stride(v)
+        kind, dtype, n, kv, dim = self._type(batch, k, "k"), k.dtype, batch.tokens, self.kv_heads, self.head_dim
+        _, k_stride = self._rows(k, n, kv, "k", dtype)
+        _, v_stride = self._rows(v, n, kv, "v", dtype)
+        heads = q_stride = out_stride = 0
+        q_at = out_at = q_bias_at = q_norm_at = turns = None
         if q is not None:
-            heads = self._rows(q, batch, 0, "q", dtype).shape[1]
+            heads, q_stride = self._rows(q, n, 0, "q", dtype)
             if out is None:
-                out = torch.empty((batch.tokens, heads, dim), dtype=dtype, device=self.device)
-            self._rows(out, batch, heads, "out", dtype)
-            r.heads, r.q, r.q_out, r.q_stride, r.q_out_stride = heads, q.data_ptr(), out.data_ptr(), self._stride(q), self._stride(out)
-            r.q_norm, r.q_bias = self._vector(q_norm, dim, "q_norm"), self._vector(q_bias, heads * dim, "q_bias")
-        r.k_norm, r.k_bias, r.v_bias = self._vector(k_norm, dim, "k_norm"), self._vector(k_bias, kv * dim, "k_bias"), self._vector(v_bias, kv * dim, "v_bias")
+                out = torch.empty((n, heads, dim), dtype=dtype, device=self.device)
+            _, out_stride = self._rows(out, n, heads, "out", dtype)
+            q_at, out_at = q.data_ptr(), out.data_ptr()
+            q_norm_at, q_bias_at = self._vector(q_norm, dim, "q_norm"), self._vector(q_bias, heads * dim, "q_bias")
+        width = adjacent = 0
+        factor = 1.0
         if rotary is not None:
-            if rotary.turns.device != self.device:
-                _fail(f"the rotation is on {rotary.turns.device}, the cache on {self.device}")
-            r.rope_turns, r.rope_dim, r.rope_adjacent, r.rope_attn_factor = rotary.turns.data_ptr(), rotary.width, rotary.adjacent, rotary.attn_factor
-        r.eps, r.type = eps, _TYPES[dtype]
-        self._call(self._lib.brisk_cuda_cache4_append, batch.c, r)
+            if rotary.turns.device != self.device or rotary.width > dim:
+                _fail(f"the rotation is of {rotary.width} values on {rotary.turns.device}, the cache's heads of {dim} on {self.device}")
+            turns, width, adjacent, factor = rotary.turns.data_ptr(), rotary.width, rotary.adjacent, rotary.attn_factor
+        rows = abi.Cache4Rows(q_at, k.data_ptr(), v.data_ptr(), out_at, q_stride, k_stride, v_stride, out_stride, q_bias_at,
+                              self._vector(k_bias, kv * dim, "k_bias"), self._vector(v_bias, kv * dim, "v_bias"), q_norm_at,
+                              self._vector(k_norm, dim, "k_norm"), turns, width, adjacent, factor, eps, heads, kind)
+        self._call(self._lib.brisk_cuda_cache4_append, batch.ref, C.byref(rows))
         return out
 
     def attention(self, batch: Batch, q, scale: float = 0.0, window: int = 0, out=None):
         """softmax(scale * q k) v of every row over the positions it sees: up to its own, with a window the last `window` of them. scale 0:
         1 / sqrt(head_dim). Rows behind the last sequence's stay as they are in `out` (unset, where it is made here)."""
-        self._check(batch)
-        heads = self._rows(q, batch, 0, "q").shape[1]
+        kind = self._type(batch, q, "q")
+        heads, q_stride = self._rows(q, batch.tokens, 0, "q", q.dtype)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        self._rows(out, batch, heads, "out", q.dtype)
+        _, out_stride = self._rows(out, batch.tokens, heads, "out", q.dtype)
         if not 0 <= window <= 0x7fffffff:
             _fail("a window is from 0 to 2^31 - 1 positions")
-        self._call(self._lib.brisk_cuda_cache4_attention, batch.c, _TYPES[q.dtype], q.data_ptr(), out.data_ptr(), self._stride(q), self._stride(out), heads,
-                   scale, window)
+        self._call(self._lib.brisk_cuda_cache4_attention, batch.ref, kind, q.data_ptr(), out.data_ptr(), q_stride, out_stride, heads, scale, window)
         return out
 
     def read(self, batch: Batch, dtype=torch.float32, k_out=None, v_out=None):
         """The stored rows at the positions of the batch's tokens, as values: two tensors [tokens, kv_heads, head_dim]."""
-        self._check(batch)
         if dtype not in _TYPES:
             _fail("a cache is read as float32, float16 or bfloat16")
-        outs = []
-        for t, what in ((k_out, "k_out"), (v_out, "v_out")):
-            t = torch.empty((batch.tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) if t is None else t
-            outs.append(self._rows(t, batch, self.kv_heads, what, dtype))
-        k, v = outs
-        self._call(self._lib.brisk_cuda_cache4_read, batch.c, _TYPES[dtype], k.data_ptr(), v.data_ptr(), self._stride(k), self._stride(v))
+        shape = (batch.tokens, self.kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device) if k_out is None else k_out
+        v = torch.empty(shape, dtype=dtype, device=self.device) if v_out is None else v_out
+        kind = self._type(batch, k, "k_out")
+        _, k_stride = self._rows(k, batch.tokens, self.kv_heads, "k_out", dtype)
+        _, v_stride = self._rows(v, batch.tokens, self.kv_heads, "v_out", dtype)
+        self._call(self._lib.brisk_cuda_cache4_read, batch.ref, kind, k.data_ptr(), v.data_ptr(), k_stride, v_stride)
         return k, v
