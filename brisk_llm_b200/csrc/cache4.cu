@@ -2,12 +2,15 @@
 // rows back as values, and the C entries of include/brisk_cuda.h. The attention over it is in cache4_attn.cu.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/brisk_cuda.h"
 #include "cache4.h"
+#include "packed.cuh"
 #include "pdl.cuh"
 
 namespace bk {
@@ -74,34 +77,58 @@ __device__ __forceinline__ float eight_bits(double v) {
     return float(__longlong_as_double((long long)(u & ~((1ull << 45) - 1))));
 }
 
-// A row of 32 E values, E to a lane, to its blocks of 32. The borders between two numbers, (n - 8.5) d with d of 8 significant bits, are
-// exact in 32 bits: the number is estimated by a reciprocal and then put right by comparing with the two borders beside it, so
-// it is the one that the definition floor(x / d + 8.5) has, whatever the estimate rounds to. NaN counts as 0 and an
-// infinity as the largest number that a block holds, so that no row of the cache holds either.
-template <class Real, int E>
-__device__ __forceinline__ void store_blocks(Real (&x)[E], uint8_t* quants, __half* scales) {
-    constexpr int kLanes = 32 / E;  // of a block
-    const uint32_t lane = threadIdx.x & 31;
+// The append kernel: a lane has 8 values of a head's row, so that a row takes D / 8 lanes and a warp 32 / (D / 8) rows at a time; four lanes
+// have a block of 32.
+constexpr int kLane = 8;
+
+// Four numbers of four bits, each to a byte.
+__device__ __forceinline__ uint32_t spread(uint32_t v) {
+    v = (v | (v << 8)) & 0x00ff00ffu;
+    return (v | (v << 4)) & 0x0f0f0f0fu;
+}
+
+// What a lane's values become: numbers of four bits, and their block's scale.
+struct Numbers {
+    uint32_t packed;
+    __half scale;
+};
+
+// The borders between two numbers, (n - 8.5) d with d of 8 significant bits, are exact in 32 bits: the number is estimated by a
+// reciprocal and then put right by comparing with the two borders beside it, so it is the one that the definition floor(x / d + 8.5)
+// has, whatever the estimate rounds to. NaN counts as 0 and an infinity as the largest number that a block holds, so that no row of
+// the cache holds either.
+// Where values may be `within` of what they stand for, *doubt says that this leaves a number or the scale open; a lane whose `within` is 0
+// has the values themselves.
+template <class Real>
+__device__ __forceinline__ Numbers to_numbers(Real (&x)[kLane], float within = 0.0f, bool* doubt = nullptr) {
     Real high = -Real(3e38f), low = Real(3e38f);
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
+    for (int j = 0; j < kLane; ++j) {
         x[j] = x[j] != x[j] ? Real(0) : x[j] > Real(3e38f) ? Real(3e38f) : x[j] < -Real(3e38f) ? -Real(3e38f) : x[j];
         high = x[j] > high ? x[j] : high;
         low = x[j] < low ? x[j] : low;
     }
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
+    for (int o = 2; o > 0; o >>= 1) {
         const Real h = __shfl_xor_sync(0xffffffffu, high, o), l = __shfl_xor_sync(0xffffffffu, low, o);
         high = h > high ? h : high;
         low = l < low ? l : low;
     }
     const Real peak = high >= -low ? high : low;
     const float wanted = peak == Real(0) ? 0.0f : eight_bits(peak * Real(-0.125));
-    const __half d = __float2half_rn(fminf(fmaxf(wanted, -65280.0f), 65280.0f));  // 255 x 256: the largest f16 of 8 bits
-    const float signed_d = __half2float(d), size = fabsf(signed_d), inverse = size != 0.0f ? __fdividef(1.0f, size) : 0.0f;
-    uint32_t packed = 0;
+    if (doubt != nullptr) {
+        float most = within;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
+        for (int o = 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float p = fabsf(float(peak));
+        *doubt = most != 0.0f && (eight_bits((p - most) * 0.125f) != eight_bits((p + most) * 0.125f) || fabsf(float(high + low)) <= 2.0f * most || !(p < 1e30f));
+    }
+    Numbers out;
+    out.scale = __float2half_rn(fminf(fmaxf(wanted, -65280.0f), 65280.0f));  // 255 x 256: the largest f16 of 8 bits
+    const float signed_d = __half2float(out.scale), size = fabsf(signed_d), inverse = size != 0.0f ? __fdividef(1.0f, size) : 0.0f;
+    out.packed = 0;
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
         float n = 8.0f;
         if (size != 0.0f) {
             const Real r = signed_d < 0.0f ? -x[j] : x[j];
@@ -109,115 +136,340 @@ __device__ __forceinline__ void store_blocks(Real (&x)[E], uint8_t* quants, __ha
             if (r < Real((n - 8.5f) * size)) n = n - 1.0f;
             else if (r >= Real((n - 7.5f) * size)) n = n + 1.0f;
             n = fminf(fmaxf(n, 0.0f), 15.0f);
+            if (doubt != nullptr && within != 0.0f) *doubt = *doubt || fabsf(float(r) - (n - 8.5f) * size) <= within || fabsf((n - 7.5f) * size - float(r)) <= within;
         }
-        packed |= uint32_t(n) << (4 * j);
+        out.packed |= uint32_t(n) << (4 * j);
     }
-    const uint32_t upper = __shfl_xor_sync(0xffffffffu, packed, kLanes / 2);  // the numbers of the values 16 further on
-    const uint32_t in_block = lane % kLanes, block = lane / kLanes;
-    if (in_block < kLanes / 2) {
-        Values<uint8_t, E> bytes;
+    return out;
+}
+
+// The same in a third of the instructions where nothing is in doubt, for values that may be `within` of what they stand for: false, and
+// nothing to be relied on, where a block has a scale that this leaves open (or that is too large or too small to divide by) or a
+// value that lies by a border.
+__device__ __forceinline__ bool quick_numbers(const float (&x)[kLane], float within, Numbers& out) {
+    float high = x[0], low = x[0], nan = 0.0f;
 #pragma unroll
-        for (int j = 0; j < E; ++j) bytes.v[j] = uint8_t(((packed >> (4 * j)) & 15u) | (((upper >> (4 * j)) & 15u) << 4));
-        *reinterpret_cast<Values<uint8_t, E>*>(quants + block * 16 + in_block * E) = bytes;
-        if (in_block == 0) scales[block] = d;
+    for (int j = 0; j < kLane; ++j) {
+        high = fmaxf(high, x[j]);
+        low = fminf(low, x[j]);
+        nan += x[j];  // or an infinity
+    }
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1) {
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        within = fmaxf(within, __shfl_xor_sync(0xffffffffu, within, o));
+    }
+    const float peak = high >= -low ? high : low, size_of_peak = fabsf(peak), d = eight_bits(peak * -0.125f);
+    const bool sure = size_of_peak < 1e5f && size_of_peak > 1e-3f && eight_bits((size_of_peak - within) * 0.125f) == eight_bits((size_of_peak + within) * 0.125f) &&
+                      (within == 0.0f || fabsf(high + low) > 2.0f * within) && nan == nan;
+    out.scale = __float2half_rn(d);
+    const float inverse = __fdividef(1.0f, d);
+    float far = 0.0f;  // of a value from the middle between two borders, in steps
+    uint32_t packed[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+        const float w = fminf(fmaxf(fmaf(x[j], inverse, 8.0f), 0.0f), 15.0f), v = w + 8388608.0f;  // to the next whole number, in the lowest bits
+        far = fmaxf(far, fabsf(w - (v - 8388608.0f)));
+        packed[j / 4] += __float_as_uint(v) << (4 * (j % 4));
+    }
+    out.packed = __byte_perm(packed[0], packed[1], 0x5410);
+    // reciprocal, product and sum are under 2^-18 of a step off (values are up to 8 steps), a value `within` of its own
+    return sure && far < 0.5f - 0x1p-18f - within * fabsf(inverse) * 1.001f;
+}
+
+// Two lanes on are the values 16 further on, the upper half of these bytes.
+__device__ __forceinline__ void store_numbers(const Numbers& y, bool there, uint8_t* quants, __half* scales) {
+    const uint32_t upper = __shfl_xor_sync(0xffffffffu, y.packed, 2), in_block = threadIdx.x & 3;
+    if (there && in_block < 2) {
+        uint2 bytes;
+        bytes.x = spread(y.packed & 0xffffu) | (spread(upper & 0xffffu) << 4);
+        bytes.y = spread(y.packed >> 16) | (spread(upper >> 16) << 4);
+        *reinterpret_cast<uint2*>(quants + in_block * 8) = bytes;
+        if (in_block == 0) *scales = y.scale;
     }
 }
 
-// y = x / rms(x) * norm, then the pairs of the first rope_dim values turned by (cos, sin). `pass` is the warp's scratch of 32 E values.
-template <class Real, int E>
-__device__ __forceinline__ void norm_and_turn(Real (&x)[E], const float* norm, float eps, uint32_t rope_dim, int adjacent, const double2* turn, Real* pass) {
+// x over its root mean square, times norm; a row is D / 8 lanes.
+template <class Real, int D>
+__device__ __forceinline__ void normed(Real (&x)[kLane], const float* norm, float eps) {
+    Real sum = Real(0);
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) sum = fused(x[j], x[j], sum);
+#pragma unroll
+    for (int o = D / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const Real scale = Real(1) / root(sum / Real(D) + Real(eps));
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) x[j] = x[j] * scale * Real(norm[j]);
+}
+
+// What a lane needs to turn its values of any row of the token: y = x c + other s, in pairs of values.
+struct Turns {
+    f32x2 c[kLane / 2], s[kLane / 2];
+    uint32_t first, rope_dim, half;  // first: the lane's place in a row, in values
+    int adjacent;
+    int from;   // the lane that has the others of this lane's pairs, where pairs fall on whole lanes
+    bool whole, turns;  // whether they do (or are side by side), and then whether this lane's values turn
+};
+
+// cosine, sine: of the token's pairs, in 32 bits.
+template <int D>
+__device__ __forceinline__ Turns turns_of(uint32_t rope_dim, int adjacent, const float* cosine, const float* sine) {
+    Turns t;
     const uint32_t lane = threadIdx.x & 31;
-    if (norm != nullptr) {
-        Real sum = Real(0);
+    t.first = (lane & (D / 8 - 1)) * kLane;
+    t.rope_dim = rope_dim;
+    t.half = rope_dim / 2;
+    t.adjacent = adjacent;
+    t.whole = rope_dim % kLane == 0 && (adjacent || t.half % kLane == 0);
+    t.turns = t.first < rope_dim;
+    t.from = int(lane) + (t.first < t.half ? int(t.half / kLane) : -int(t.half / kLane));
+    if (t.whole && !adjacent) {
+        const bool is_first = t.first < t.half;
+        const uint32_t at = t.turns ? is_first ? t.first : t.first - t.half : 0;
 #pragma unroll
-        for (int j = 0; j < E; ++j) sum = fused(x[j], x[j], sum);
+        for (int j = 0; j < kLane; j += 4) {
+            const float4 c = *reinterpret_cast<const float4*>(cosine + at + j), s = *reinterpret_cast<const float4*>(sine + at + j);
+            t.c[j / 2] = pack2(c.x, c.y);
+            t.c[j / 2 + 1] = pack2(c.z, c.w);
+            t.s[j / 2] = is_first ? pack2(-s.x, -s.y) : pack2(s.x, s.y);
+            t.s[j / 2 + 1] = is_first ? pack2(-s.z, -s.w) : pack2(s.z, s.w);
+        }
+    } else if (adjacent) {
+        const uint32_t at = t.turns ? t.first / 2 : 0;  // the table has kLane values more than pairs
+        const float4 c = *reinterpret_cast<const float4*>(cosine + at), s = *reinterpret_cast<const float4*>(sine + at);
+        t.c[0] = pack2(c.x, c.x); t.c[1] = pack2(c.y, c.y); t.c[2] = pack2(c.z, c.z); t.c[3] = pack2(c.w, c.w);
+        t.s[0] = pack2(-s.x, s.x); t.s[1] = pack2(-s.y, s.y); t.s[2] = pack2(-s.z, s.z); t.s[3] = pack2(-s.w, s.w);
+    } else {
+        float c[kLane], s[kLane];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const Real scale = Real(1) / root(sum / Real(32 * E) + Real(eps));
+        for (int j = 0; j < kLane; ++j) {
+            const uint32_t i = t.first + j;
+            c[j] = i < t.half ? cosine[i] : i < rope_dim ? cosine[i - t.half] : 1.0f;
+            s[j] = i < t.half ? -sine[i] : i < rope_dim ? sine[i - t.half] : 0.0f;
+        }
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = x[j] * scale * Real(norm[lane * E + j]);
+        for (int j = 0; j < kLane / 2; ++j) {
+            t.c[j] = pack2(c[2 * j], c[2 * j + 1]);
+            t.s[j] = pack2(s[2 * j], s[2 * j + 1]);
+        }
     }
-    if (rope_dim == 0) return;
-    const uint32_t half = rope_dim / 2;
-    if (!adjacent) {
+    return t;
+}
+
+// Turns the lane's values; `pass`: the warp's scratch of 256 values. Returns (BOUND) the lane's largest sum of the magnitudes of a pair, 0
+// where its values do not turn.
+template <bool BOUND>
+__device__ __forceinline__ float turned(float (&x)[kLane], const Turns& t, float* pass) {
+    const uint32_t lane = threadIdx.x & 31, row = lane * kLane - t.first;
+    float other[kLane], most = 0.0f;
+    if (t.adjacent) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) other[j] = x[j ^ 1];
+    } else if (t.whole) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) other[j] = __shfl_sync(0xffffffffu, x[j], t.from);
+    } else {
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < E; ++j) pass[lane * E + j] = x[j];
+        for (int j = 0; j < kLane; ++j) pass[lane * kLane + j] = x[j];
         __syncwarp();
-    }
-    Real y[E];
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const uint32_t i = lane * E + j;
+        for (int j = 0; j < kLane; ++j) {
+            const uint32_t i = t.first + j;
+            other[j] = i < t.half ? pass[row + i + t.half] : i < t.rope_dim ? pass[row + i - t.half] : 0.0f;
+        }
+    }
+    if (t.whole) {
+        if (t.turns) {
+#pragma unroll
+            for (int j = 0; j < kLane / 2; ++j) {
+                if (BOUND) most = fmaxf(most, fmaxf(fabsf(x[2 * j]) + fabsf(other[2 * j]), fabsf(x[2 * j + 1]) + fabsf(other[2 * j + 1])));
+                unpack2(fma2(pack2(x[2 * j], x[2 * j + 1]), t.c[j], mul2(pack2(other[2 * j], other[2 * j + 1]), t.s[j])), x[2 * j], x[2 * j + 1]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            if (t.first + j < t.rope_dim) {
+                float c, s, c1, s1;
+                unpack2(t.c[j / 2], c, c1);
+                unpack2(t.s[j / 2], s, s1);
+                most = fmaxf(most, fabsf(x[j]) + fabsf(other[j]));
+                x[j] = fmaf(x[j], j % 2 ? c1 : c, other[j] * (j % 2 ? s1 : s));
+            }
+        }
+    }
+    return most;
+}
+
+// Keys' or values' rows in 64 bits.
+template <class T, int D>
+__device__ __noinline__ Numbers exact_numbers(const T* src, int wide, const float* bias, const float* norm, float eps, uint32_t first, uint32_t rope_dim, int adjacent, const double2* turn,
+                                              double* pass) {
+    const uint32_t lane = threadIdx.x & 31, half = rope_dim / 2, row = lane * kLane - first;
+    float in[kLane];
+    double x[kLane], y[kLane];
+    load_values<T, kLane>(src, wide, in);
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) x[j] = bias != nullptr ? double(in[j]) + double(bias[j]) : double(in[j]);
+    if (norm != nullptr) normed<double, D>(x, norm, eps);
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) pass[lane * kLane + j] = x[j];
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) {
+        const uint32_t i = first + j;
         y[j] = x[j];
         if (i < rope_dim) {
-            const bool first = adjacent ? j % 2 == 0 : i < half;
-            const double2 t = turn[adjacent ? i / 2 : first ? i : i - half];
-            const Real c = Real(t.x), s = Real(t.y);
-            const Real other = adjacent ? x[j ^ 1] : pass[first ? i + half : i - half];
-            y[j] = first ? fused(x[j], c, -(other * s)) : fused(other, s, x[j] * c);
+            const bool is_first = adjacent ? j % 2 == 0 : i < half;
+            const double2 t = turn[adjacent ? i / 2 : is_first ? i : i - half];
+            const double other = pass[row + (adjacent ? i ^ 1 : is_first ? i + half : i - half)];
+            y[j] = is_first ? fma(x[j], t.x, -(other * t.y)) : fma(other, t.y, x[j] * t.x);
         }
     }
-#pragma unroll
-    for (int j = 0; j < E; ++j) x[j] = y[j];
+    return to_numbers<double>(y);
 }
 
-// A warp to a head's row of q, k or v; a CTA of eight warps to some of a token's rows, so that the token's angles are made once for
-// them. Angles, and the keys' norm, rotation and borders, are in 64 bits: a far position turns a pair thousands of times, and a
-// key that lies next to the border between two numbers is stored as the definition has it, not as 32 bits happen to round.
-template <class T, int E>
-__global__ void __launch_bounds__(256) cache4_append_kernel(const Cache4 c, const Cache4Batch b, const Cache4Append a, uint32_t rows_per_cta) {
-    __shared__ double2 turn[E * 16];
-    __shared__ double pass[8][E * 32];
+constexpr int kAppendWarps = 2;
+
+// A CTA of two warps to some of a token's rows, so that the token's angles are made once for them, in 64 bits: a far position turns a pair
+// thousands of times. A warp takes 32 / (D / 8) rows of q, of k or of v at a time. What is stored is what 64 bits give: a row is computed
+// in 32, with a bound on how far its values may be off, and once more in 64 where that bound reaches a border between two numbers or
+// two scales (a row in some hundreds). The bound, in half-ulps 2^-24 of the sum of a pair's magnitudes: bias 1, mean of squares
+// (8 + 5 + 1) / 2, root and quotient 2, two products 2, cos and sin and their sum 3: at most 15.
+//
+// Rows are asked for first of all, so that they arrive while the angles are made; the loop then finds them in shared memory.
+template <class T, int D>
+__global__ void __launch_bounds__(32 * kAppendWarps, 12) cache4_append_kernel(const Cache4 c, const Cache4Batch b, const Cache4Append a, uint32_t items_per_cta) {
+    constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // lanes of a row, rows of a warp
+    constexpr int kPieces = int(sizeof(T)) * kLane / 16, kAhead = 4;  // 16-byte pieces of a lane's values; items asked for at a time
+    __shared__ double2 turn[D / 2];
+    __shared__ __align__(16) float cosine[D / 2 + kLane], sine[D / 2 + kLane];
+    __shared__ double pass[kAppendWarps][256];
+    __shared__ uint4 asked[kAppendWarps][kAhead][kPieces][32];
     wait_for_previous();
     release_next();
-    const uint32_t row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = (lane & (kLanes - 1)) * kLane;
+    const uint32_t q_items = (a.heads + kRows - 1) / kRows, kv_items = (c.kv_heads + kRows - 1) / kRows, end = min(q_items + 2 * kv_items, (blockIdx.y + 1) * items_per_cta);
+    const T* q = static_cast<const T*>(a.q) + size_t(row) * a.q_stride + first;
+    const T* k = static_cast<const T*>(a.k) + size_t(row) * a.k_stride + first;
+    const T* v = static_cast<const T*>(a.v) + size_t(row) * a.v_stride + first;
+    // The last rows of a warp may be of no head: they repeat the last one's, and store nothing.
+    auto source_of = [&](uint32_t item) {
+        const uint32_t which = item < q_items ? item : item < q_items + kv_items ? item - q_items : item - q_items - kv_items;
+        return (item < q_items ? q : item < q_items + kv_items ? k : v) + min(which * kRows + lane / kLanes, (item < q_items ? a.heads : c.kv_heads) - 1) * D;
+    };
+    auto ask = [&](uint32_t item) {
+        if (a.wide) {
+#pragma unroll
+            for (int n = 0; n < kAhead; ++n) {
+                const uint32_t x = item + n * kAppendWarps;
+                if (x < end) {
+                    const T* src = source_of(x);
+#pragma unroll
+                    for (int p = 0; p < kPieces; ++p) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(&asked[warp][n][p][lane]))), "l"(src + p * (kLane / kPieces)) : "memory");
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    uint32_t item = blockIdx.y * items_per_cta + warp;
+    ask(item);
     uint32_t sequence;
     long long position;
-    if (!row_place(b, row, sequence, position)) return;
-    for (uint32_t i = threadIdx.x; i < a.rope_dim / 2; i += 256) {
+    const bool ours = row_place(b, row, sequence, position);
+    if (!ours) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        return;
+    }
+    for (uint32_t i = threadIdx.x; i < a.rope_dim / 2; i += 32 * kAppendWarps) {
         double angle = double(position) * a.turns[i], z, w;
         angle -= rint(angle);
         sincospi(2.0 * angle, &z, &w);
-        turn[i] = make_double2(w * double(a.attn_factor), z * double(a.attn_factor));
+        w *= double(a.attn_factor);
+        z *= double(a.attn_factor);
+        turn[i] = make_double2(w, z);
+        cosine[i] = float(w);
+        sine[i] = float(z);
     }
-    __syncthreads();
     const uint32_t column = uint32_t(position >> c.page_shift), slot = uint32_t(position) & (c.page_size - 1);
     const bool held = position >= 0 && position < (long long)b.columns * c.page_size;
     const int32_t page = held ? page_of(c, b, sequence, column) : -1;
-    const uint32_t all = a.heads + 2 * c.kv_heads, end = min(all, (blockIdx.y + 1) * rows_per_cta);
-    for (uint32_t r = blockIdx.y * rows_per_cta + warp; r < end; r += 8) {
-        const bool is_q = r < a.heads, is_k = !is_q && r < a.heads + c.kv_heads;
-        const uint32_t head = is_q ? r : is_k ? r - a.heads : r - a.heads - c.kv_heads;
-        if (!is_q && page < 0) continue;
-        const size_t at = size_t(head) * (32 * E) + lane * E;
-        const T* src = is_q ? static_cast<const T*>(a.q) + size_t(row) * a.q_stride : is_k ? static_cast<const T*>(a.k) + size_t(row) * a.k_stride
-                                                                                   : static_cast<const T*>(a.v) + size_t(row) * a.v_stride;
-        const float* bias = is_q ? a.q_bias : is_k ? a.k_bias : a.v_bias;
-        float in[E];
-        load_values<T, E>(src + at, a.wide, in);
-        if (is_q) {
-            if (bias != nullptr) {
+    const size_t page_block = ((size_t(max(page, 0)) * c.kv_heads) * c.page_size + slot) * (D / 32) + first / 32;
+    __syncthreads();
+    const Turns t = turns_of<D>(a.rope_dim, a.adjacent, cosine, sine);
+    const float reach = 0x1p-20f * fmaxf(1.0f, fabsf(a.attn_factor));
+    T* q_out = static_cast<T*>(a.q_out) + size_t(row) * a.q_out_stride + first;
+    const uint32_t sub = lane / kLanes;
+    // Rows of queries (kind 0), keys (1) or values (2): item `which` of its kind, the n-th that was asked for.
+    auto take = [&](auto kind, uint32_t which, uint32_t n) {
+        constexpr int kKind = decltype(kind)::value;
+        const uint32_t heads = kKind == 0 ? a.heads : c.kv_heads, wanted = which * kRows + sub, head = min(wanted, heads - 1);
+        const bool there = wanted < heads;
+        const T* src = (kKind == 0 ? q : kKind == 1 ? k : v) + head * D;
+        float x[kLane];
+        if (a.wide) {
+            Values<T, kLane> u;
 #pragma unroll
-                for (int j = 0; j < E; ++j) in[j] += bias[at + j];
-            }
-            norm_and_turn<float, E>(in, a.q_norm, a.eps, a.rope_dim, a.adjacent, turn, reinterpret_cast<float*>(pass[warp]));
-            store_values<T, E>(static_cast<T*>(a.q_out) + size_t(row) * a.q_out_stride + at, a.wide, in);
-            continue;
-        }
-        const size_t stored = ((size_t(page) * c.kv_heads + head) * c.page_size + slot) * E;  // in units of dim / E = 32 values
-        double x[E];
+            for (int p = 0; p < kPieces; ++p) reinterpret_cast<uint4*>(&u)[p] = asked[warp][n][p][lane];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x[j] = bias != nullptr ? double(in[j]) + double(bias[at + j]) : double(in[j]);
-        if (is_k) {
-            norm_and_turn<double, E>(x, a.k_norm, a.eps, a.rope_dim, a.adjacent, turn, pass[warp]);
-            store_blocks<double, E>(x, c.k_quants + stored * 16, c.k_scales + stored);
-        } else if (bias != nullptr) {
-            store_blocks<double, E>(x, c.v_quants + stored * 16, c.v_scales + stored);
+            for (int j = 0; j < kLane; ++j) x[j] = Convert<T>::from(u.v[j]);
         } else {
-            store_blocks<float, E>(in, c.v_quants + stored * 16, c.v_scales + stored);
+            load_values<T, kLane>(src, 0, x);
+        }
+        const float* bias = kKind == 0 ? a.q_bias : kKind == 1 ? a.k_bias : a.v_bias;
+        const float* norm = kKind == 0 ? a.q_norm : kKind == 1 ? a.k_norm : nullptr;
+        if (bias != nullptr) {
+            bias += head * D + first;
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) x[j] = x[j] + bias[j];
+        }
+        if (kKind != 2 && norm != nullptr) {
+            norm += first;
+            normed<float, D>(x, norm, a.eps);
+        }
+        if constexpr (kKind == 0) {
+            if (a.rope_dim != 0) turned<false>(x, t, reinterpret_cast<float*>(pass[warp]));
+            if (there) store_values<T, kLane>(q_out + head * D, a.wide, x);
+        } else {
+            if (page < 0) return;
+            float most = 0.0f;
+            if (bias != nullptr || (kKind == 1 && norm != nullptr)) {
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) most = fmaxf(most, fabsf(x[j]));
+            }
+            if (kKind == 1 && a.rope_dim != 0) most = fmaxf(most, turned<true>(x, t, reinterpret_cast<float*>(pass[warp])));
+            // 0 where 32 bits hold the values themselves
+            const float within = most * reach;
+            const size_t block = page_block + size_t(head) * c.page_size * (D / 32);
+            Numbers numbers;
+            const bool sure = quick_numbers(x, within, numbers);
+            if (__any_sync(0xffffffffu, !sure)) {
+                bool doubt;
+                numbers = to_numbers<float>(x, within, &doubt);
+                if (__any_sync(0xffffffffu, doubt)) {
+                    numbers = exact_numbers<T, D>(src, a.wide, bias, norm, a.eps, first, kKind == 1 ? a.rope_dim : 0, a.adjacent, turn, pass[warp]);
+                }
+            }
+            store_numbers(numbers, there, (kKind == 1 ? c.k_quants : c.v_quants) + block * 16, (kKind == 1 ? c.k_scales : c.v_scales) + block);
+        }
+    };
+    for (uint32_t n = 0; item < end; item += kAppendWarps) {
+        if (n == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (item < q_items) take(std::integral_constant<int, 0>{}, item, n);
+        else if (item < q_items + kv_items) take(std::integral_constant<int, 1>{}, item - q_items, n);
+        else take(std::integral_constant<int, 2>{}, item - q_items - kv_items, n);
+        if (++n == kAhead) {
+            n = 0;
+            __syncwarp();
+            ask(item + kAppendWarps);
         }
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // A warp to a head's row.
@@ -251,26 +503,28 @@ __global__ void __launch_bounds__(256) cache4_read_kernel(const Cache4 c, const 
     }
 }
 
-template <class T, int E>
+template <class T, int D>
 void append_typed(const Cache4& c, const Cache4Batch& b, const Cache4Append& a, bool dependent, cudaStream_t s) {
-    // Few tokens: a warp per row, so that a call is as short as its slowest row. Many: a CTA per token, which makes the angles once.
-    const uint32_t all = a.heads + 2 * c.kv_heads;
-    const uint32_t parts = b.tokens >= 592 ? 1 : (all + 7) / 8;
-    const uint32_t rows_per_cta = (all + parts - 1) / parts;
-    const dim3 grid(b.tokens, (all + rows_per_cta - 1) / rows_per_cta);
+    // Few tokens: an item to a warp, so that a call is as short as its slowest row. Many: a CTA to a token, which makes the angles once (setting
+    // up is half a row's work; 6600 tokens of 30 heads in two warps 55 us, in four 69).
+    constexpr uint32_t kRows = 32 / (D / 8);
+    const uint32_t items = (a.heads + kRows - 1) / kRows + 2 * ((c.kv_heads + kRows - 1) / kRows);
+    const uint32_t most = (items + kAppendWarps - 1) / kAppendWarps, parts = std::max(1u, std::min(most, 2368u / b.tokens));
+    const uint32_t items_per_cta = (items + parts - 1) / parts;
+    const dim3 grid(b.tokens, (items + items_per_cta - 1) / items_per_cta);
     if (dependent) {
-        launch_dependent(cache4_append_kernel<T, E>, grid, dim3(256), 0, s, c, b, a, rows_per_cta);
+        launch_dependent(cache4_append_kernel<T, D>, grid, dim3(32 * kAppendWarps), 0, s, c, b, a, items_per_cta);
     } else {
-        cache4_append_kernel<T, E><<<grid, 256, 0, s>>>(c, b, a, rows_per_cta);
+        cache4_append_kernel<T, D><<<grid, 32 * kAppendWarps, 0, s>>>(c, b, a, items_per_cta);
         BK_CUDA(cudaGetLastError());
     }
 }
 
 template <class T>
 void append_sized(const Cache4& c, const Cache4Batch& b, const Cache4Append& a, bool dependent, cudaStream_t s) {
-    if (c.dim == 64) append_typed<T, 2>(c, b, a, dependent, s);
-    else if (c.dim == 128) append_typed<T, 4>(c, b, a, dependent, s);
-    else append_typed<T, 8>(c, b, a, dependent, s);
+    if (c.dim == 64) append_typed<T, 64>(c, b, a, dependent, s);
+    else if (c.dim == 128) append_typed<T, 128>(c, b, a, dependent, s);
+    else append_typed<T, 256>(c, b, a, dependent, s);
 }
 
 template <class T>
@@ -291,10 +545,10 @@ uint32_t type_bytes(int type) { return type == T_F32 ? 4 : 2; }
 
 void launch_cache4_append(const Cache4& c, const Cache4Batch& b, const Cache4Append& in, int type, bool dependent, cudaStream_t s) {
     Cache4Append a = in;
-    const uintptr_t size = type_bytes(type), lane = uintptr_t(c.dim / 32) * size, step = lane > 16 ? 16 : lane;
+    const uintptr_t size = type_bytes(type);
     uintptr_t all = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | (a.k_stride * size) | (a.v_stride * size);
     if (a.heads != 0) all |= reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.q_out) | (a.q_stride * size) | (a.q_out_stride * size);
-    a.wide = all % step == 0;
+    a.wide = all % 16 == 0;
     if (type == T_F32) append_sized<float>(c, b, a, dependent, s);
     else if (type == T_F16) append_sized<__half>(c, b, a, dependent, s);
     else append_sized<__nv_bfloat16>(c, b, a, dependent, s);

@@ -79,6 +79,7 @@ __device__ __forceinline__ bool row_place(const Cache4Batch& b, uint32_t row, ui
     } else {
         const uint32_t lane = threadIdx.x & 31;
         uint32_t before = 0;  // sequences that end at or before the row
+#pragma unroll 4
         for (uint32_t s = 0; s < b.sequences; s += 32) {
             const bool ended = s + lane < b.sequences && b.query_start[s + lane + 1] <= int32_t(row);
             before += __popc(__ballot_sync(0xffffffffu, ended));
