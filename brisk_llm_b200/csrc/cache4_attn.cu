@@ -90,6 +90,8 @@ template <int D, int NT, int W, bool TWO> struct Split {
     static constexpr int kStages = D == 64 ? 4 : 3;
     static constexpr int kRow = D / 2, kScales = D / 16;  // bytes of a position
     static constexpr int kK = 0, kV = kTile * kRow, kKs = 2 * kTile * kRow, kVs = kKs + kTile * kScales, kStage = kVs + kTile * kScales;
+    static constexpr int kOrdered = kThreads < 128 ? kThreads : 128;  // sequences that are put in order
+    static constexpr uint32_t kManyCtas = 296;
     static constexpr int kPitch = D + 4;  // floats between two rows of a warp's result
     static constexpr int kSteps = D / 16;
     static constexpr bool kHeld = NT == 1 && !TWO && D <= 128;  // the queries stay in registers
@@ -147,7 +149,26 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t S = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t unit = blockIdx.x / S, kv = unit % c.kv_heads, tile = unit / c.kv_heads, sequence = blockIdx.y;
+    const uint32_t unit = blockIdx.x / S, kv = unit % c.kv_heads, tile = unit / c.kv_heads;
+    uint32_t sequence = blockIdx.y;
+    if (gridDim.y > 1 && gridDim.y <= uint32_t(G::kOrdered) && gridDim.x * gridDim.y > G::kManyCtas) {
+        // Ragged sequences and more CTAs than fit at a time: the longest go first, so that none begins when the others are done. Every CTA finds
+        // the sequence of its place for itself (one token of 64 sequences of up to 8000 positions 107 -> 83 us).
+        int* length = reinterpret_cast<int*>(smem);  // the rings are empty yet
+        uint32_t* chosen = reinterpret_cast<uint32_t*>(length + G::kOrdered);
+        if (tid < gridDim.y) length[tid] = b.context[tid];
+        __syncthreads();
+        if (tid < gridDim.y) {
+            const int mine = length[tid];
+            uint32_t before = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < gridDim.y; ++i) before += length[i] > mine || (length[i] == mine && i < tid);
+            if (before == blockIdx.y) *chosen = tid;
+        }
+        __syncthreads();
+        sequence = *chosen;
+        __syncthreads();
+    }
     const uint32_t group = a.heads / c.kv_heads;
     const long long context = b.context[sequence];
     uint32_t first_row, count;
@@ -640,24 +661,28 @@ void attend_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, 
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads), tiles = (rows + 8 * NT - 1) / (8 * NT);
     const uint64_t units = tiles * c.kv_heads * b.sequences;
     const uint64_t length = a.window != 0 ? std::min<uint64_t>(b.max_length, uint64_t(a.window) + 8 * NT + 31) : b.max_length;
-    // Clusters grow while there are CTAs to spare (two to an SM for up to 8 rows; those of more rows, with an SM's shared memory to
-    // themselves, to half the SMs, past which clusters wait for room) and a tile for every warp. us at S = 1, 2, 4, 8, 16: one token
-    // of 8 key/value heads at 517 positions 8.0 7.8 6.5 6.5 7.5, at 32 767 192 107 56 33 27, of 64 x 8 at 8000 107 106 117 165 297; 36 rows
-    // of 8 heads at 2064 44 30 21 31 37. Four or sixteen warps a CTA are no faster at any of them.
+    // Clusters grow while that gives the SMs CTAs (about four thirds for each with 8 rows; one for every second with 16, whose rings leave
+    // no room for another) and every warp tiles: one, for 16 CTAs four. us at S = 1, 2, 4, 8, 16: one token of 8 key/value heads at 517
+    // positions 8.0 7.8 6.5 6.5 7.5, at 32 767 192 107 56 33 27; 36 rows of 8 heads at 2064 20 15 14 19 24; 20 rows at 8000 50 30 18 16 21.
+    // Four or sixteen warps a CTA are no faster at any of them.
     constexpr int kWarps = D == 256 ? 4 : 8;
-    const uint64_t most = NT == 1 ? 2 * multiprocessors() : multiprocessors() / 2;
+    const uint64_t most = NT == 1 ? multiprocessors() * 4 / 3 : multiprocessors() / 2;
     uint32_t split = 1;
-    while (split < 16 && units * split * 2 <= most && length > uint64_t(split) * kWarps * 32) split *= 2;
+    while (split < 16 && units * split * 2 <= most && length > uint64_t(split) * kWarps * (split < 8 ? 32 : 128)) split *= 2;
     if (units / b.sequences * split > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
     launch_split<T, D, NT, kWarps>(c, b, a, units, split, dependent, s);
 }
 
+// 8 rows to a CTA, two of which an SM holds, or 16, which share the keys and values they widen: where there are CTAs enough all the same. us
+// with 8 / 16: 9 tokens of 32 heads after 2064 positions 12 / 12, 24 tokens after 8000 46 / 63, 64 after 2000 26 / 21, 128 after 4000 83 /
+// 67; 600 tokens in heads of 256 41 / 53. With 32 a CTA has an SM to itself and is slower than either nearly everywhere.
 template <class T, int D>
 void attend_sized(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, bool dependent, cudaStream_t s) {
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
-    if (rows <= 8) attend_split<T, D, 1>(c, b, a, dependent, s);
-    else if (rows <= 16 || D == 256) attend_split<T, D, 2>(c, b, a, dependent, s);
-    else if constexpr (D < 256) attend_split<T, D, 4>(c, b, a, dependent, s);
+    if constexpr (D <= 128) {
+        if (rows >= 64 && (rows + 7) / 8 * c.kv_heads * b.sequences >= 256) return attend_split<T, D, 2>(c, b, a, dependent, s);
+    }
+    attend_split<T, D, 1>(c, b, a, dependent, s);
 }
 
 template <class T>

@@ -607,10 +607,11 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
 
 }  // namespace
 
-// A CTA of this kernel takes its positions one after another, about 2 us for 128 of them and up to 128 rows; the kernel of few rows takes 32 rows
-// at a time and spreads their positions. So this one needs rows enough for that to cost the other more: per sequence and
-// key/value head over 32, and 160 times 32 rows in all. us of few / many rows, bf16 heads of 128 after 2000 to 4000 positions: 128 x 32 rows 54 / 76
-// and 32 / 41, 192 x 32 61 / 42, 256 x 32 86 / 67, 512 x 32 167 / 68; f32 43 / 50, 79 / 95, 84 / 53, 127 / 83.
+// A CTA of this kernel takes its positions one after another, about 2 us for 128 of them and up to 128 rows; the kernel of few rows takes 8 or 16
+// rows at a time and spreads their positions. So this one needs rows enough for that to cost the other more: per sequence and
+// key/value head over 32, and 160 times 32 rows in all. us of few / many rows, bf16 heads of 128: 128 times 32 rows after 2000 to 4000 positions
+// 67 / 76 and 38 / 41, 192 times 60 / 42, 256 times 32 at the start of a prompt 20 / 12, 512 times 36 after 3000 140 / 119; f32 89 / 96, 48 / 53,
+// 78 / 56, 23 / 16, 183 / 156.
 bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a) {
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
     return c.dim <= 128 && rows > 32 && (rows + 31) / 32 * c.kv_heads * b.sequences >= 160;
