@@ -168,7 +168,7 @@ class PagedCache:
         if q is not None:
             heads, q_stride = self._rows(q, n, 0, "q", dtype)
             if out is None:
-                out = torch.empty((n, heads, dim), dtype=dtype, device=self.device)
+                out = q.new_empty((n, heads, dim))
             _, out_stride = self._rows(out, n, heads, "out", dtype)
             q_at, out_at = q.data_ptr(), out.data_ptr()
             q_norm_at, q_bias_at = self._vector(q_norm, dim, "q_norm"), self._vector(q_bias, heads * dim, "q_bias")
@@ -190,7 +190,7 @@ class PagedCache:
         kind = self._type(batch, q, "q")
         heads, q_stride = self._rows(q, batch.tokens, 0, "q", q.dtype)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+            out = q.new_empty(q.shape)
         _, out_stride = self._rows(out, batch.tokens, heads, "out", q.dtype)
         if not 0 <= window <= 0x7fffffff:
             _fail("a window is from 0 to 2^31 - 1 positions")

@@ -123,7 +123,7 @@ template <int D, bool TWO> struct Prompt {
     static constexpr int kFlush = 4, kTotal = kO + D;
 };
 constexpr int kByPolynomial = 1;  // of four pairs
-constexpr int kPromptThreads = 16 * 32;
+constexpr int kPromptThreads = 16 * 32, kOrdered = 128;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -152,7 +152,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     wait_for_previous();
-    const uint32_t group = a.heads / c.kv_heads, sequence = blockIdx.y, kv = blockIdx.x % c.kv_heads;
+    uint32_t sequence = blockIdx.y;
+    if (gridDim.y > 1 && gridDim.y <= uint32_t(kOrdered)) {  // the longest sequences begin first (see cache4_attn.cu)
+        int* length = reinterpret_cast<int*>(smem);
+        uint32_t* chosen = reinterpret_cast<uint32_t*>(length + kOrdered);
+        if (tid < gridDim.y) {
+            uint32_t from, tokens;
+            sequence_rows(b, tid, from, tokens);
+            length[tid] = int(min((long long)b.context[tid] + tokens, 0x7fffffffll));
+        }
+        __syncthreads();
+        if (tid < gridDim.y) {
+            const int mine = length[tid];
+            uint32_t before = 0;
+#pragma unroll 8
+            for (uint32_t i = 0; i < gridDim.y; ++i) before += length[i] > mine || (length[i] == mine && i < tid);
+            if (before == blockIdx.y) *chosen = tid;
+        }
+        __syncthreads();
+        sequence = *chosen;
+        __syncthreads();
+    }
+    const uint32_t group = a.heads / c.kv_heads, kv = blockIdx.x % c.kv_heads;
     const uint32_t tile = gridDim.x / c.kv_heads - 1 - blockIdx.x / c.kv_heads;  // the last rows, which see most, begin first
     const long long context = b.context[sequence], held = (long long)b.columns * c.page_size;
     uint32_t first_row, count;
