@@ -666,7 +666,8 @@ extern "C" int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const br
         require((rows->k_stride >= kv && rows->v_stride >= kv), "needs token strides of at least a token's heads (k, v)");
         require(rows->rope_dim <= c.dim && rows->rope_dim % 2 == 0, "rotates an even width of at most the head size");
         require(rows->rope_dim == 0 || rows->rope_turns != nullptr, "needs the turns of the pairs it rotates");
-        require(rows->eps >= 0.0f, "needs an epsilon of at least 0");
+        require(rows->eps >= 0.0f && std::isfinite(rows->eps), "needs a finite epsilon of at least 0");
+        require(std::isfinite(rows->rope_attn_factor), "needs a finite factor on cos and sin");
         bk::Cache4Append a;
         a.q = rows->q; a.k = rows->k; a.v = rows->v; a.q_out = rows->q_out;
         a.q_stride = rows->q_stride; a.k_stride = rows->k_stride; a.v_stride = rows->v_stride; a.q_out_stride = rows->q_out_stride;
@@ -702,6 +703,7 @@ extern "C" int brisk_cuda_cache4_attention(const brisk_cuda_cache4* cache, const
         bk::check_type(type);
         require(heads != 0 && heads <= 65535 && heads % c.kv_heads == 0, "needs a number of query heads that is a multiple of its key/value heads");
         require(std::isfinite(scale), "needs a finite scale");
+        require(uint64_t(batch->tokens) * (heads / c.kv_heads) <= 0x7fffffffull, "takes up to 2^31 - 1 tokens times query heads of a key/value head");
         if (b.tokens == 0) return;
         const uintptr_t size = type == bk::T_F32 ? 4 : 2;
         require(q != nullptr && out != nullptr && bk::aligned(q, size) && bk::aligned(out, size), "needs queries, and where the result goes, on boundaries of their type");

@@ -6,6 +6,8 @@
 // product - 3 bits and a sign times 8 - is an f16 number: kernels that multiply in f16 multiply the stored values themselves.
 #pragma once
 
+#include <mutex>
+
 #include "common.cuh"
 
 namespace bk {
@@ -45,6 +47,18 @@ struct Cache4Attend {
     uint32_t heads = 0, window = 0;
     float scale = 0.0f;
     int wide = 0;
+};
+
+// What a kernel needs set once for each device (its opt-in to shared memory and cluster sizes), before its first launch there, whichever of
+// the host's threads comes first.
+struct DeviceSetup {
+    std::once_flag flags[64];
+    template <class Fn> void once(Fn&& fn) {
+        int device = 0;
+        BK_CUDA(cudaGetDevice(&device));
+        if (device < 0 || device >= 64) throw CudaError("cuda: device ordinal out of range");
+        std::call_once(flags[device], fn);
+    }
 };
 
 // type: T_F32, T_F16 or T_BF16, of q, k, v and what comes out. dependent: started by launch_dependent().

@@ -635,11 +635,11 @@ void launch_split(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, 
     using G = Split<D, NT, W, sizeof(T) == 4>;
     const auto kernel = cache4_split_kernel<T, D, NT, W>;
     static_assert(G::kBytes <= 227 * 1024);
-    static DeviceOnce once;
-    if (once.first()) {
+    static DeviceSetup setup;
+    setup.once([&] {
         BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(G::kBytes)));
         BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    }
+    });
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(uint32_t(units / b.sequences * split), b.sequences);
     cfg.blockDim = dim3(32 * W);

@@ -607,8 +607,8 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
     const auto kernel = cache4_prompt_kernel<T, D>;
     constexpr size_t smem = Prompt<D, sizeof(T) == 4>::kBytes;
     static_assert(smem <= 227 * 1024);
-    static DeviceOnce once;
-    if (once.first()) BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+    static DeviceSetup setup;
+    setup.once([&] { BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem))); });
     Cache4Attend a = in;
     a.wide = (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (a.q_stride * sizeof(T)) | (a.out_stride * sizeof(T))) % 16 == 0;
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);

@@ -271,8 +271,10 @@ int brisk_cuda_argmax_static(const float* logits, uint32_t vocab, uint32_t rows,
  * several sequences, or of long ones, in 28 % of the f16 bytes: rows are appended, attended to and read back by the three calls below.
  * Sessions created with BRISK_CUDA_FLAG_CACHE_4BIT run their layers over them. All pointers are DEVICE pointers on the current device unless
  * they are said to be host ones; `stream` is a cudaStream_t (NULL: the default stream). The calls launch on the stream and return: no
- * allocation, no synchronisation, no workspace, nothing kept - they may be captured into a graph and replayed, with context,
- * page_table and query_start read at every replay. They return 0, or -1 and a message in err before anything is launched.
+ * allocation, no synchronisation, no workspace, nothing kept. So calls may overlap on several streams and from several threads as long as
+ * none writes what another reads, and they may be captured into a graph and replayed, with context, page_table and query_start read at
+ * every replay (make one call of the kind before the capture: the driver loads kernels when they are first used). They return 0, or -1
+ * and a message in err before anything is launched.
  *
  * A head's row of one position is head_dim / 32 blocks of 32 values: a scale d, and 16 bytes in the order of a Q4_0 block (byte j: value j
  * in the low, value j + 16 in the high four bits); a value is (n - 8) d. Appending chooses d = -m / 8, m the block's value of largest
@@ -293,8 +295,8 @@ typedef struct brisk_cuda_cache4 {
 /* Tokens of several sequences one behind the other: token i of sequence s is row query_start[s] + i of q, k, v and the outputs and
  * stands at position context[s] + i. Rows behind the last sequence's are not touched; a sequence may have no tokens, and no positions
  * before them. A page number outside the pool is no error: its positions are not written and read as rows of zeros; so are positions
- * past the table's columns, which attention does not see at all. Two columns of the sequences that append to one page, at the same
- * position, leave either's row. */
+ * past the table's columns, which attention does not see at all. What two tokens of a batch leave at one place of one page - a page that
+ * stands in two columns - is not defined. */
 typedef struct brisk_cuda_cache4_batch {
     const int32_t* context;     /* [sequences] positions before this batch's tokens                                        */
     const int32_t* page_table;  /* [sequences][table_columns]; NULL: column c of sequence s is page s * table_columns + c   */

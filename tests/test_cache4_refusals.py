@@ -68,7 +68,7 @@ def test_a_batch_that_does_not_hold_is_refused(wrong, message):
     (dict(type=2), "f32, f16 and bf16"), (dict(k=None), "keys and values"), (dict(v=P + 1), "boundaries"), (dict(heads=3), "multiple"),
     (dict(q=None), "queries"), (dict(q_out=P + 1), "queries"), (dict(q_stride=511), "strides"), (dict(q_out_stride=0), "strides"), (dict(k_stride=255), "strides"),
     (dict(v_stride=128), "strides"), (dict(rope_dim=130), "even width"), (dict(rope_dim=63), "even width"), (dict(rope_turns=None), "turns"),
-    (dict(eps=-1.0), "epsilon"), (dict(eps=float("nan")), "epsilon")])
+    (dict(eps=-1.0), "epsilon"), (dict(eps=float("nan")), "epsilon"), (dict(rope_attn_factor=float("inf")), "factor")])
 def test_rows_that_do_not_fit_are_refused(wrong, message):
     rc, text = append(cache(), batch(), rows(**wrong))
     assert rc != 0 and message in text
@@ -80,6 +80,11 @@ def test_rows_that_do_not_fit_are_refused(wrong, message):
 def test_an_attention_that_does_not_fit_is_refused(wrong, message):
     rc, text = attention(cache(), batch(), **wrong)
     assert rc != 0 and message in text
+
+
+def test_more_rows_than_an_index_holds_are_refused():
+    rc, text = attention(cache(kv_heads=1, head_dim=64), batch(tokens=1 << 20), q_stride=1 << 20, out_stride=1 << 20, heads=4096)
+    assert rc != 0 and "2^31" in text
 
 
 def test_a_read_that_does_not_fit_is_refused():

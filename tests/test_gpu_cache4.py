@@ -393,6 +393,34 @@ def test_captured_and_replayed_on_two_streams(tokens):
             assert torch.equal(want, out)  # the same call on the same data: bit for bit
 
 
+def test_calls_of_several_threads_at_once():
+    """Each thread with a stream and a batch of its own, over one cache that they read and pages of their own that they append to."""
+    import threading
+
+    import torch
+    from brisk_llm_b200 import cache4
+    worlds = [World(20 + i, 2, 128, [400 + 10 * i, 30], [t, t]) for i, t in enumerate((1, 9, 340, 1))]
+    rotary = cache4.Rotary(128, 1e6)
+    inputs = [[torch.randn((w.rows, h, 128), device="cuda") for h in (8, 2, 2)] for w in worlds]
+    want = [w.cache.attention(w.batch, w.cache.append(w.batch, *x, rotary=rotary)) for w, x in zip(worlds, inputs)]
+    torch.cuda.synchronize()
+    got = [None] * len(worlds)
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i] = worlds[i].cache.attention(worlds[i].batch, worlds[i].cache.append(worlds[i].batch, *inputs[i], rotary=rotary))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(worlds))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_results_do_not_depend_on_the_run():
     import torch
     for tokens in (1, 9, 300):
