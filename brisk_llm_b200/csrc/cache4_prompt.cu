@@ -39,25 +39,6 @@ __device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4
 }
 
 __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
-// 2^x of a pair without the special-function unit, which the weights of two tiles would keep busier than their products keep the
-// tensor cores: the integer part by adding 1.5 x 2^23, 2^r for r in [-1/2, 1/2] by the polynomial of degree 4 with the least
-// relative error (Remez: 2.6e-6, a hundredth of what rounding the weight to f16 costs), the integer into the exponent.
-__device__ __forceinline__ void exp2_by_polynomial(f32x2 x, float& y, float& z) {
-    float a, b;
-    unpack2(x, a, b);
-    x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-    const f32x2 magic = pack2(12582912.0f, 12582912.0f), t = add2(x, magic), r = sub2(x, sub2(t, magic));
-    f32x2 p = fma2(r, pack2(0.0095701f, 0.0095701f), pack2(0.05591786f, 0.05591786f));
-    p = fma2(p, r, pack2(0.24024745f, 0.24024745f));
-    p = fma2(p, r, pack2(0.69312181f, 0.69312181f));
-    p = fma2(p, r, pack2(0.99999926f, 0.99999926f));
-    float ta, tb, pa, pb;
-    unpack2(t, ta, tb);
-    unpack2(p, pa, pb);
-    y = __uint_as_float((__float_as_uint(ta) << 23) + __float_as_uint(pa));
-    z = __uint_as_float((__float_as_uint(tb) << 23) + __float_as_uint(pb));
-}
-
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool accumulate) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"(uint32_t(accumulate)) : "memory");
 }
@@ -122,7 +103,6 @@ template <int D, bool TWO> struct Prompt {
     // those sums with rounding, in the columns of the second tile of rows, which f32 does without.
     static constexpr int kFlush = 4, kTotal = kO + D;
 };
-constexpr int kByPolynomial = 1;  // of four pairs
 constexpr int kPromptThreads = 16 * 32, kOrdered = 128;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -333,32 +313,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 const float less = m == -INFINITY ? 0.0f : -m;
                 const f32x2 scale2 = pack2(scale, scale), less2 = pack2(less, less);
                 f32x2 sum[4] = {pack2(l, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-                auto weights = [&](auto all) {
 #pragma unroll
-                    for (int ch = 0; ch < kN / 32; ++ch) {
-                        uint32_t w[16], w_low[16];
+                for (int ch = 0; ch < kN / 32; ++ch) {
+                    uint32_t w[16], w_low[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const f32x2 v = fma2(pack2(x[ch][2 * i], x[ch][2 * i + 1]), scale2, less2);
-                            float y, z;
-                            if (decltype(all)::value && i % 4 < kByPolynomial) {
-                                exp2_by_polynomial(v, y, z);
-                            } else {
-                                unpack2(v, y, z);
-                                y = exp2_fast(y);
-                                z = exp2_fast(z);
-                            }
-                            sum[i & 3] = add2(sum[i & 3], pack2(y, z));
-                            const __half2 h = __floats2half2_rn(y, z);
-                            w[i] = bits(h);
-                            if (kTwo) w_low[i] = bits(__floats2half2_rn(y - __low2float(h), z - __high2float(h)));
-                        }
-                        tmem_st16(w_at + ch * 16, w);
-                        if (kTwo) tmem_st16(w_at + kN / 2 + ch * 16, w_low);
+                    for (int i = 0; i < 16; ++i) {
+                        float y, z;
+                        unpack2(fma2(pack2(x[ch][2 * i], x[ch][2 * i + 1]), scale2, less2), y, z);
+                        y = exp2_fast(y);
+                        z = exp2_fast(z);
+                        sum[i & 3] = add2(sum[i & 3], pack2(y, z));
+                        const __half2 h = __floats2half2_rn(y, z);
+                        w[i] = bits(h);
+                        if (kTwo) w_low[i] = bits(__floats2half2_rn(y - __low2float(h), z - __high2float(h)));
                     }
-                };
-                if (whole && !kTwo) weights(std::true_type{});
-                else weights(std::false_type{});
+                    tmem_st16(w_at + ch * 16, w);
+                    if (kTwo) tmem_st16(w_at + kN / 2 + ch * 16, w_low);
+                }
                 float even, odd;
                 unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), even, odd);
                 l = even + odd;
