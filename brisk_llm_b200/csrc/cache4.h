@@ -66,7 +66,7 @@ void launch_cache4_append(const Cache4& c, const Cache4Batch& b, const Cache4App
 void launch_cache4_read(const Cache4& c, const Cache4Batch& b, void* k_out, void* v_out, size_t k_stride, size_t v_stride, int type, cudaStream_t s);
 void launch_cache4_attention(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s);
 // The kernel of many rows (cache4_prompt.cu), and whether launch_cache4_attention takes it.
-bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a);
+bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type);
 void launch_cache4_prompt(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s);
 
 #ifdef __CUDACC__

@@ -695,7 +695,7 @@ void attend(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, bool d
 }  // namespace
 
 void launch_cache4_attention(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s) {
-    if (cache4_prompt_takes(c, b, a)) launch_cache4_prompt(c, b, a, type, dependent, s);
+    if (cache4_prompt_takes(c, b, a, type)) launch_cache4_prompt(c, b, a, type, dependent, s);
     else if (type == T_F32) attend<float>(c, b, a, dependent, s);
     else if (type == T_F16) attend<__half>(c, b, a, dependent, s);
     else attend<__nv_bfloat16>(c, b, a, dependent, s);

@@ -1,4 +1,5 @@
 // Attention over the paged cache in 4 bits for many rows - prompts and their chunks - on the tensor cores of tensor memory.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -12,6 +13,12 @@
 
 namespace bk {
 namespace {
+
+namespace cg = cooperative_groups;
+
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
@@ -104,6 +111,7 @@ template <int D, bool TWO> struct Prompt {
     static constexpr int kFlush = 4, kTotal = kO + D;
 };
 constexpr int kPromptThreads = 16 * 32, kOrdered = 128;
+constexpr uint32_t kMostSplits = 4;
 template <int N> __device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
@@ -119,6 +127,7 @@ struct Bars {
 //     S = Q K^T (both operands in shared memory),     O += P V (P in tensor memory, where the softmax wrote it over S).
 // The head's values lie in Q and K in the order in which a 4-bit word yields them. V is widened with neighbouring positions side by side, as
 // the product wants them: two words of two positions give pairs of one dim.
+// Where rows are few for the SMs, up to four CTAs of a cluster share a row's positions and join at the end.
 // Every wait is bounded; one that runs out leaves NaN in the rows of its tile.
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a, uint32_t rows_per_cta) {
@@ -153,8 +162,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
         sequence = *chosen;
         __syncthreads();
     }
-    const uint32_t group = a.heads / c.kv_heads, kv = blockIdx.x % c.kv_heads;
-    const uint32_t tile = gridDim.x / c.kv_heads - 1 - blockIdx.x / c.kv_heads;  // the last rows, which see most, begin first
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t S = cluster.num_blocks(), rank = cluster.block_rank();  // CTAs that share the positions of these rows
+    const uint32_t group = a.heads / c.kv_heads, kv = blockIdx.x / S % c.kv_heads;
+    const uint32_t tile = gridDim.x / S / c.kv_heads - 1 - blockIdx.x / S / c.kv_heads;  // the last rows, which see most, begin first
     const long long context = b.context[sequence], held = (long long)b.columns * c.page_size;
     uint32_t first_row, count;
     sequence_rows(b, sequence, first_row, count);
@@ -190,7 +201,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     auto last_of = [&](uint32_t token) { return int(max(min(context + token, held - 1), -1ll)); };
     auto first_of = [&](uint32_t token) { return a.window != 0 ? int(min(max(context + token - (long long)a.window + 1, 0ll), held)) : 0; };
     const int lo = first_of(row0 / group), hi = last_of((row0 + rows - 1) / group);
-    const int begin = lo & ~(kN - 1), tiles = hi >= lo ? (hi - begin) / kN + 1 : 0, halves_used = rows > 128 ? 2 : 1;
+    const int all_tiles = hi >= lo ? (hi - (lo & ~(kN - 1))) / kN + 1 : 0, halves_used = rows > 128 ? 2 : 1;
+    const int each = (all_tiles + int(S) - 1) / int(S), before = min(int(rank) * each, all_tiles), tiles = min(each, all_tiles - before);
+    const int begin = (lo & ~(kN - 1)) + before * kN;
     const long long limit = kTcWaitCycles;
     bool dead = bar->tmem != 0;
 
@@ -201,7 +214,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
         const bool real = half * 128 + r < rows;
         const uint32_t token = real ? row / group : 0, head = row - token * group;
         T* out = static_cast<T*>(a.out) + size_t(first_row + token) * a.out_stride + size_t(kv * group + head) * D;
-        if (int(half) < halves_used && tiles != 0) {
+        const bool works = int(half) < halves_used && tiles != 0;
+        const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
+        const uint32_t o_at = lanes + G::kO + half * D;
+        float m = -INFINITY, l = 0.0f;
+        if (works) {
             // the row's queries: a power of two brings the largest to 2^10 (see cache4_attn.cu)
             Row<T, D> q;
             q.load(static_cast<const T*>(a.q) + size_t(first_row + token) * a.q_stride + size_t(kv * group + head) * D, real, a.wide);
@@ -237,8 +254,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             const int last = real ? last_of(token) : -1, first = real ? first_of(token) : 0;
             const uint32_t last_row = min(row0 + half * 128 + 127, row0 + rows - 1);
             const int whole_to = last_of((row0 + half * 128) / group), whole_from = first_of(last_row / group);
-            const uint32_t lanes = tmem + ((warp & 3) << 21);  // this warp's 32 lanes
-            const uint32_t s_at = lanes, w_at = lanes + G::kW + half * 64, o_at = lanes + G::kO + half * D;
+            const uint32_t s_at = lanes, w_at = lanes + G::kW + half * 64;
             auto scale_columns = [&](uint32_t at, float by) {
 #pragma unroll
                 for (int ch = 0; ch < D / 16; ++ch) {
@@ -265,7 +281,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 }
                 tmem_wait_st();
             };
-            float m = -INFINITY, l = 0.0f;
             for (int j = 0; j < tiles; ++j) {
                 mbar_wait(&bar->s_full[half], j & 1, dead, limit);
                 dead = __any_sync(0xffffffffu, dead);
@@ -341,37 +356,106 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             if (!dead) mbar_wait(&bar->o_done[half], (tiles - 1) & 1, dead, limit);
             dead = __any_sync(0xffffffffu, dead);
             tc_fence_after();
-            const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
-#pragma unroll
-            for (int ch = 0; ch < D / 32; ++ch) {
-                uint32_t x[32];
-                tmem_ld32(o_at + ch * 32, x);
+        }
+        // 32 values of the row's result, before they are divided by the sum of its weights
+        auto result_of = [&](int ch, uint32_t (&x)[32]) {
+            tmem_ld32(o_at + ch * 32, x);
+            tmem_wait_ld();
+            if (kTwo && tiles > G::kFlush) {
+                uint32_t y[32];
+                tmem_ld32(lanes + G::kTotal + ch * 32, y);
                 tmem_wait_ld();
-                if (kTwo && tiles > G::kFlush) {
-                    uint32_t y[32];
-                    tmem_ld32(lanes + G::kTotal + ch * 32, y);
-                    tmem_wait_ld();
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
-                }
-                if (real) {
-                    if (a.wide) {
-                        constexpr int kPer = 16 / sizeof(T);
+                for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
+            }
+        };
+        if (S == 1) {
+            if (works) {
+                const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
-                        for (int i = 0; i < 32; i += kPer) {
-                            alignas(16) T y[kPer];
+                for (int ch = 0; ch < D / 32; ++ch) {
+                    uint32_t x[32];
+                    result_of(ch, x);
+                    if (real) {
+                        if (a.wide) {
+                            constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-                            for (int u = 0; u < kPer; ++u) put(y + u, __uint_as_float(x[i + u]) * inverse);
-                            *reinterpret_cast<uint4*>(out + ch * 32 + i) = *reinterpret_cast<const uint4*>(y);
+                            for (int i = 0; i < 32; i += kPer) {
+                                alignas(16) T y[kPer];
+#pragma unroll
+                                for (int u = 0; u < kPer; ++u) put(y + u, __uint_as_float(x[i + u]) * inverse);
+                                *reinterpret_cast<uint4*>(out + ch * 32 + i) = *reinterpret_cast<const uint4*>(y);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) put(out + ch * 32 + i, __uint_as_float(x[i]) * inverse);
                         }
-                    } else {
+                    }
+                }
+            } else if (real && tiles == 0) {  // rows that see nothing
+                for (int i = 0; i < D; ++i) put(out + i, 0.0f);
+            }
+        } else {
+            // Every CTA sums D / S values of each row: the others write theirs, with their maximum and sum, where its operand tiles were.
+            const uint32_t share = D / S, at = half * 128 + r;
+            uint4* received = reinterpret_cast<uint4*>(smem);            // [S][share / 4][256]
+            float2* sums = reinterpret_cast<float2*>(smem + 256 * D * 4);  // [S][256] of maximum and sum
+            static_assert(256 * D * 4 + kMostSplits * 256 * 8 <= G::kBarriersAt);
+            cluster_meet();  // nobody's products read operand tiles any more
+            if (int(half) < halves_used) {
+                for (uint32_t k = 0; k < S; ++k) *cluster.map_shared_rank(sums + rank * 256 + at, k) = dead ? make_float2(0.0f, __int_as_float(0x7fc00000)) : make_float2(m, l);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) put(out + ch * 32 + i, __uint_as_float(x[i]) * inverse);
+                for (int ch = 0; ch < D / 32; ++ch) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = 0;
+                    if (works) result_of(ch, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        const uint32_t dim = ch * 32 + i;
+                        *cluster.map_shared_rank(received + (rank * (share / 4) + dim % share / 4) * 256 + at, dim / share) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
                     }
                 }
             }
-        } else if (real && tiles == 0) {  // rows that see nothing
-            for (int i = 0; i < D; ++i) put(out + i, 0.0f);
+            cluster_meet();
+            if (real) {
+                float most = -INFINITY, sum = 0.0f, by[kMostSplits];
+                for (uint32_t k = 0; k < S; ++k) most = fmaxf(most, sums[k * 256 + at].x);
+#pragma unroll
+                for (uint32_t k = 0; k < kMostSplits; ++k) {
+                    by[k] = 0.0f;
+                    if (k < S) {
+                        const float2 y = sums[k * 256 + at];
+                        by[k] = y.x == -INFINITY ? 0.0f : exp2_fast(y.x - most);
+                        sum = fmaf(y.y, by[k], sum);
+                    }
+                }
+                const float inverse = sum == 0.0f ? 0.0f : __fdiv_rn(1.0f, sum);
+                for (uint32_t i = 0; i < share; i += 4) {
+                    float x[4] = {};
+#pragma unroll
+                    for (uint32_t k = 0; k < kMostSplits; ++k) {
+                        if (k < S) {
+                            const uint4 y = received[(k * (share / 4) + i / 4) * 256 + at];
+                            x[0] = fmaf(__uint_as_float(y.x), by[k], x[0]);
+                            x[1] = fmaf(__uint_as_float(y.y), by[k], x[1]);
+                            x[2] = fmaf(__uint_as_float(y.z), by[k], x[2]);
+                            x[3] = fmaf(__uint_as_float(y.w), by[k], x[3]);
+                        }
+                    }
+                    alignas(16) T z[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) put(z + u, x[u] * inverse);
+                    T* dst = out + rank * share + i;
+                    if (a.wide) {
+                        using Four = std::conditional_t<kTwo, uint4, uint2>;
+                        *reinterpret_cast<Four*>(dst) = *reinterpret_cast<const Four*>(z);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) dst[u] = z[u];
+                    }
+                }
+            }
         }
     } else if (warp < 12) {
         // ---- keys and values: 4 bits to f16 operand tiles ----
@@ -557,6 +641,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             mbar_drain(&bar->drained, 0);
         }
     }
+    if (warp >= 8 && S > 1) {
+        __syncwarp();
+        cluster_meet();
+        cluster_meet();
+    }
     release_next();
     __syncwarp();
     tc_fence_before();
@@ -573,6 +662,28 @@ uint32_t multiprocessors() {
     return uint32_t(count);
 }
 
+// How a call's rows and positions are shared out.
+struct Shares {
+    uint32_t rows_per_cta, split;
+    uint64_t ctas, length;  // of a sequence, where one CTA has all its positions; positions that a tile of rows sees at most
+};
+Shares shares_of(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, bool two) {
+    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads), sms = multiprocessors();
+    Shares x;
+    // Two tiles of rows share their keys and values where there are CTAs for all SMs all the same. us with 128 / 256 rows a CTA, bf16 heads
+    // of 128: 512 tokens of 32 heads (128 or 64 CTAs) 17 / 20, 3000 positions further on 68 / 79; 16 sequences of 64 tokens after 1000 (256
+    // or 128) 56 / 37.
+    x.rows_per_cta = !two && (rows + 127) / 128 * c.kv_heads * b.sequences > sms ? 256 : 128;
+    x.ctas = (rows + x.rows_per_cta - 1) / x.rows_per_cta * c.kv_heads;
+    x.length = a.window != 0 ? std::min<uint64_t>(b.max_length, uint64_t(a.window) + x.rows_per_cta) : b.max_length;
+    // Positions are spread while SMs are free for it and a CTA keeps some tiles: joining costs 3 us. us with 1 / 2 / 4 CTAs, bf16 heads of 128:
+    // 32 tiles of rows after 4000 positions 77 / 46 / 31, 64 of them 79 / 48 / 59 (256 CTAs are two rounds); at the start of a prompt, 512 positions
+    // at most, 16.4 / 16.1 / 28.
+    x.split = 1;
+    while (x.split < kMostSplits && x.ctas * b.sequences * x.split * 2 <= sms && x.length > uint64_t(x.split) * (two ? 256 : 512)) x.split *= 2;
+    return x;
+}
+
 template <class T, int D>
 void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in, bool dependent, cudaStream_t s) {
     const auto kernel = cache4_prompt_kernel<T, D>;
@@ -582,31 +693,39 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
     setup.once([&] { BK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem))); });
     Cache4Attend a = in;
     a.wide = (reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out) | (a.q_stride * sizeof(T)) | (a.out_stride * sizeof(T))) % 16 == 0;
-    const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
-    // Two tiles of rows share their keys and values where there are CTAs for all SMs all the same. us with 128 / 256 rows a CTA, bf16 heads
-    // of 128: 512 tokens of 32 heads (128 or 64 CTAs) 17 / 20, 3000 positions further on 68 / 79; 16 sequences of 64 tokens after 1000 (256
-    // or 128) 56 / 37.
-    const uint32_t rows_per_cta = sizeof(T) < 4 && (rows + 127) / 128 * c.kv_heads * b.sequences > multiprocessors() ? 256 : 128;
-    const uint64_t grid = (rows + rows_per_cta - 1) / rows_per_cta * c.kv_heads;
-    if (grid > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
-    if (dependent) {
-        launch_dependent(kernel, dim3(uint32_t(grid), b.sequences), dim3(kPromptThreads), smem, s, c, b, a, rows_per_cta);
-    } else {
-        kernel<<<dim3(uint32_t(grid), b.sequences), kPromptThreads, smem, s>>>(c, b, a, rows_per_cta);
-        BK_CUDA(cudaGetLastError());
-    }
+    const Shares x = shares_of(c, b, a, sizeof(T) == 4);
+    if (x.ctas * x.split > 0x7fffffffull) throw CudaError("cuda: the 4-bit cache's attention takes fewer rows than these");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(uint32_t(x.ctas * x.split), b.sequences);
+    cfg.blockDim = dim3(kPromptThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = x.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 2 : 1;
+    BK_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, b, a, x.rows_per_cta));
 }
 
 }  // namespace
 
-// A CTA of this kernel takes its positions one after another, about 2 us for 128 of them and up to 128 rows; the kernel of few rows takes 8 or 16
-// rows at a time and spreads their positions. So this one needs rows enough for that to cost the other more: per sequence and
-// key/value head over 32, and 160 times 32 rows in all. us of few / many rows, bf16 heads of 128: 128 times 32 rows after 2000 to 4000 positions
-// 67 / 76 and 38 / 41, 192 times 60 / 42, 256 times 32 at the start of a prompt 20 / 12, 512 times 36 after 3000 140 / 119; f32 89 / 96, 48 / 53,
-// 78 / 56, 23 / 16, 183 / 156.
-bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a) {
+// The kernel of few rows takes 16 at a time and spreads their positions over all SMs; a CTA of this one takes up to 256 rows and its positions one
+// after another. So this one needs rows enough, and the line is where the times of the two meet, in ns with bf16 heads of 128 (the other types and
+// heads move both alike): 30 and 1 for 17 positions of every 16 rows there, 10000 and 16 for a position of each round of CTAs here. us of few / many
+// rows: 64 times 32 rows after 2000 positions 21.2 / 21.0, after 8000 63 / 44, 128 times 32 after 4000 66 / 31, 256 times 32 at the start of a
+// prompt 23 / 12, 32 sequences of 36 rows after 3000 140 / 120, 8 of 18 after 2000 25 / 29; f32 27 / 25, 86 / 54, 89 / 38, 25 / 16, 183 / 157, 32 / 34.
+// With 32 rows or fewer most of a tile is empty: 32 sequences of 18 rows after 3000 96 / 121, f32 124 / 155.
+bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type) {
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
-    return c.dim <= 128 && rows > 32 && (rows + 31) / 32 * c.kv_heads * b.sequences >= 160;
+    if (c.dim > 128 || rows <= 32) return false;
+    const Shares x = shares_of(c, b, a, type == T_F32);
+    const uint64_t sms = multiprocessors(), rounds = (x.ctas * x.split * b.sequences + sms - 1) / sms;
+    const double few = double((rows + 15) / 16 * c.kv_heads * b.sequences) * (30.0 + double(x.length) / 17.0), many = 10000.0 + double(rounds) * double(x.length) * 16.0 / x.split;
+    return many < few;
 }
 
 void launch_cache4_prompt(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type, bool dependent, cudaStream_t s) {

@@ -236,6 +236,12 @@ ATTENDS = [
     (21, 3, 64, [100], [300], 16, 0),
     (32, 8, 128, [0, 100, 5], [256, 200, 301], 32, 0),
     (56, 8, 64, [31, 0], [290, 150], 64, 70),
+    # positions enough for two or four CTAs to share them; of a short sequence some of these have none
+    (8, 2, 128, [2500], [300], 64, 0),
+    (7, 1, 64, [3100], [260], 32, 0),
+    (16, 2, 128, [1999], [280], 64, 1200),
+    (16, 2, 128, [3000, 0, 0], [150, 1, 20], 16, 0),
+    (48, 3, 64, [2600, 0, 700], [70, 0, 33], 128, 0),
 ]
 
 
