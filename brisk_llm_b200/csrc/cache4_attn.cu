@@ -80,8 +80,15 @@ __device__ __forceinline__ void as_they_are(uint32_t w, uint32_t (&v)[4]) {
     v[3] = u & 0x00f000f0u;
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// .aligned: by whole warps
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // W warps a CTA, 8 NT rows, f32 (two f16 parts) or not.
 template <int D, int NT, int W, bool TWO> struct Split {

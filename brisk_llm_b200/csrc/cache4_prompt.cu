@@ -17,6 +17,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 __device__ __forceinline__ void cluster_meet() {
+    __syncwarp();  // .aligned: by whole warps
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -194,6 +195,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     }
     tc_fence_before();
     __syncthreads();
+    __syncwarp();
     tc_fence_after();
     // All 512 columns are this CTA's, so they begin at 0: as a constant the address costs the products no move between registers.
     constexpr uint32_t tmem = 0;
@@ -250,6 +252,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             async_proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->q_full[half]);
+            __syncwarp();
 
             const int last = real ? last_of(token) : -1, first = real ? first_of(token) : 0;
             const uint32_t last_row = min(row0 + half * 128 + 127, row0 + rows - 1);
@@ -282,12 +285,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 tmem_wait_st();
             };
             for (int j = 0; j < tiles; ++j) {
-                mbar_wait(&bar->s_full[half], j & 1, dead, limit);
-                dead = __any_sync(0xffffffffu, dead);
+                mbar_wait_warp(&bar->s_full[half], j & 1, dead, limit);
                 if (dead) break;
                 tc_fence_after();
                 // the last tile's scores: nobody reads these keys any more
                 if (int(half) == halves_used - 1 && (tid & 127) == 0) mbar_arrive(&bar->k_free[j & 1]);
+                __syncwarp();  // loads and stores of tensor memory are a whole warp's
                 const int base = begin + j * kN;
                 const bool whole = base + kN - 1 <= whole_to && base >= whole_from;
                 // tensor memory gives a warp little more than 32 bytes a cycle: the scores are read once and stay in registers
@@ -298,6 +301,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->s_free);
+                __syncwarp();
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < kN; ++i) {
@@ -309,11 +313,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 for (int i = 0; i < kN; i += 2) tops[i / 2 % 4] = fmaxf(tops[i / 2 % 4], fmaxf(__uint_as_float(x[i / 32][i % 32]), __uint_as_float(x[i / 32][i % 32 + 1])));
                 const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * scale;
                 if (j > 0) {  // the last weights have been read, the result is at rest
-                    mbar_wait(&bar->o_done[half], (j - 1) & 1, dead, limit);
-                    dead = __any_sync(0xffffffffu, dead);
+                    mbar_wait_warp(&bar->o_done[half], (j - 1) & 1, dead, limit);
                     if (dead) break;
                     tc_fence_after();
                     if (int(half) == halves_used - 1 && (tid & 127) == 0) mbar_arrive(&bar->v_free[(j - 1) & 1]);
+                    __syncwarp();
                     if (kTwo && j % G::kFlush == 0) add_up(j > G::kFlush);
                 }
                 // the maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do
@@ -353,8 +357,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar->p_full[half]);
             }
-            if (!dead) mbar_wait(&bar->o_done[half], (tiles - 1) & 1, dead, limit);
-            dead = __any_sync(0xffffffffu, dead);
+            mbar_wait_warp(&bar->o_done[half], (tiles - 1) & 1, dead, limit);
             tc_fence_after();
         }
         // 32 values of the row's result, before they are divided by the sum of its weights
@@ -391,10 +394,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                             for (int i = 0; i < 32; ++i) put(out + ch * 32 + i, __uint_as_float(x[i]) * inverse);
                         }
                     }
+                    __syncwarp();
                 }
             } else if (real && tiles == 0) {  // rows that see nothing
                 for (int i = 0; i < D; ++i) put(out + i, 0.0f);
             }
+            __syncwarp();
         } else {
             // Every CTA sums D / S values of each row: the others write theirs, with their maximum and sum, where its operand tiles were.
             const uint32_t share = D / S, at = half * 128 + r;
@@ -518,8 +523,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
         ask_pages(1);
         for (int j = 0; j < tiles; ++j) {
             const uint32_t slot = j & 1;
-            if (j >= 2) mbar_wait(&bar->k_free[slot], (j >> 1) - 1 & 1, dead, limit);
-            dead = __any_sync(0xffffffffu, dead);
+            if (j >= 2) mbar_wait_warp(&bar->k_free[slot], (j >> 1) - 1 & 1, dead, limit);
             if (dead) break;
             unsigned char* tile_k = smem + G::kKAt + slot * G::kK;
 #pragma unroll
@@ -539,8 +543,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             if (lane == 0) mbar_arrive(&bar->k_full[slot]);
             if (j + 1 < tiles) load_keys(j + 1);
 
-            if (j >= 2) mbar_wait(&bar->v_free[slot], (j >> 1) - 1 & 1, dead, limit);
-            dead = __any_sync(0xffffffffu, dead);
+            if (j >= 2) mbar_wait_warp(&bar->v_free[slot], (j >> 1) - 1 & 1, dead, limit);
             if (dead) break;
             unsigned char* tile_v = smem + G::kVAt + slot * G::kV;
             if (has_values) {
@@ -578,10 +581,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             const bool leader = elect_one();
             // descriptors count in 16 bytes; what is added to them is a constant, or the slot's
             const uint64_t q_desc = smem_desc_swizzled(smem_at), k_desc = smem_desc_swizzled(smem_at + G::kKAt), v_desc = smem_desc_swizzled(smem_at + G::kVAt);
-            auto wait = [&](uint64_t* x, uint32_t parity) {
-                if (!dead) mbar_wait(x, parity, dead, limit);
-                dead = __any_sync(0xffffffffu, dead);
-            };
+            auto wait = [&](uint64_t* x, uint32_t parity) { mbar_wait_warp(x, parity, dead, limit); };
             auto scores = [&](auto half, uint64_t k) {  // S = Q_i K^T
                 constexpr int i = decltype(half)::value;
                 tc_fence_after();
@@ -651,6 +651,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     tc_fence_before();
     __syncthreads();
     if (warp == 12) {
+        __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }

@@ -46,6 +46,12 @@ __device__ __forceinline__ void mbar_wait(uint64_t* b, uint32_t parity, bool& de
         }
     }
 }
+// The same by a whole warp: `dead` in every lane where one gave up, and the warp is whole behind it.
+__device__ __forceinline__ void mbar_wait_warp(uint64_t* b, uint32_t parity, bool& dead, long long limit) {
+    mbar_wait(b, parity, dead, limit);
+    dead = __any_sync(0xffffffffu, dead);
+    __syncwarp();
+}
 // A warp waits for several barriers at once, lanes first .. end - 1 for one each: even where the barriers are long
 // complete one wait costs 71 cycles, several at once 111. Every try is voted on, so that all lanes have one answer. False: gave up.
 __device__ __forceinline__ bool mbar_wait_all(uint64_t* mine, uint32_t parity, uint32_t first, uint32_t end, long long limit) {
