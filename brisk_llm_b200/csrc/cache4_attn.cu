@@ -1,11 +1,10 @@
 // Attention over the paged cache in 4 bits, for few rows: single tokens, verify steps, and whatever cache4_prompt.cu leaves.
 #include <cooperative_groups.h>
-#include <cuda_bf16.h>
 
 #include <algorithm>
 #include <cmath>
 
-#include "cache4.h"
+#include "cache4_math.cuh"
 #include "pdl.cuh"
 
 namespace bk {
@@ -13,18 +12,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -40,8 +27,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {  // an 8 x 8 matrix
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(v));
     return y;
 }
-__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
-__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
 // 16 bytes to shared memory; zeros where !there (src is then any valid address).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
@@ -50,19 +35,7 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// The eight numbers of a word, n - 8 times the scale, as four pairs: (low of bytes 0, 2), (high of 0, 2), (low of 1, 3), (high of 1, 3).
-// A number set into the mantissa of 1024 (or, 16 times it, of 1024) is exact, so is n - 8, and so is the product with a scale of 8
-// bits: three instructions a pair and no rounding.
-__device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4]) {
-    const uint32_t magic = 0x64006400u, u = w >> 8;
-    const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72
-    v[0] = bits(__hmul2(__hsub2(halves((w & 0x000f000fu) | magic), bias), scale));
-    v[1] = bits(__hmul2(__hfma2(halves((w & 0x00f000f0u) | magic), sixteenth, less), scale));
-    v[2] = bits(__hmul2(__hsub2(halves((u & 0x000f000fu) | magic), bias), scale));
-    v[3] = bits(__hmul2(__hfma2(halves((u & 0x00f000f0u) | magic), sixteenth, less), scale));
-}
-
-// The same eight numbers without a scale.
+// The eight numbers of a word (see widen) without a scale.
 __device__ __forceinline__ void centred(uint32_t w, uint32_t (&v)[4]) {
     const uint32_t magic = 0x64006400u, u = w >> 8;
     const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72
@@ -629,12 +602,6 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
         for (uint32_t k = 0; k < S; ++k) sum = fmaf(received[k * share + x], tops[k * kRows + r], sum);
         if (r < rows) put(row_of(r) + dim_of((rank * share + x) % D), sum * row_scale[r]);
     }
-}
-
-uint32_t multiprocessors() {
-    int dev = 0, count = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
-    return uint32_t(count);
 }
 
 template <class T, int D, int NT, int W>

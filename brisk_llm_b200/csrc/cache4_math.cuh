@@ -1,0 +1,45 @@
+// Helpers of the two attentions over the cache in 4 bits.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include "cache4.h"
+
+namespace bk {
+
+inline uint32_t multiprocessors() {
+    int dev = 0, count = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, dev);
+    return uint32_t(count);
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
+__device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
+
+// The eight numbers of a word, n - 8 times the scale, as four pairs: (low of bytes 0, 2), (high of 0, 2), (low of 1, 3), (high of 1, 3).
+// A number set into the mantissa of 1024 (or, 16 times it, of 1024) is exact, so is n - 8, and so is the product with a scale of 8
+// bits: three instructions a pair and no rounding.
+__device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4]) {
+    const uint32_t magic = 0x64006400u, u = w >> 8;
+    const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72
+    v[0] = bits(__hmul2(__hsub2(halves((w & 0x000f000fu) | magic), bias), scale));
+    v[1] = bits(__hmul2(__hfma2(halves((w & 0x00f000f0u) | magic), sixteenth, less), scale));
+    v[2] = bits(__hmul2(__hsub2(halves((u & 0x000f000fu) | magic), bias), scale));
+    v[3] = bits(__hmul2(__hfma2(halves((u & 0x00f000f0u) | magic), sixteenth, less), scale));
+}
+#endif
+
+}  // namespace bk
