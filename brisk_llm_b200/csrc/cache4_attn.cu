@@ -101,7 +101,7 @@ template <int D> __device__ __forceinline__ uint32_t position_of(uint32_t g) {  
 }
 
 // softmax(q k) v for 8 NT rows - tokens times the query heads of one key/value head - of one sequence. A cluster of CTAs shares the
-// positions, each warp takes tiles of 32 of them with a running maximum and sum of its own; the warps' results are joined in
+// positions, each warp takes tiles of 32 of them with a running level (of the maximum) and sum of its own; the warps' results are joined in
 // shared memory, the CTAs' over the cluster's. Positions are the rows (M) and queries the columns (N = 8) of both products,
 //     S^T = K Q^T (16 positions x 8 queries),     O^T = V^T P^T (16 dims x 8 queries),
 // so that eight query heads fill an instruction and the 4-bit words become its A operand in registers, straight from the
@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                 }
             }
         }
-        // The maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do.
+        // The level (see Level) moves only where a weight would no longer fit.
         bool above = false;
         float top[NT][2];
 #pragma unroll
@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 top[n][e] = fmaxf(fmaxf(s[0][n][e], s[0][n][2 + e]), fmaxf(s[1][n][e], s[1][n][2 + e]));
-                above = above || top[n][e] > m[n][e] + 8.0f;
+                above = above || top[n][e] > m[n][e] + Level<kTwo>::kMost;
             }
         }
         if (__any_sync(0xffffffffu, above)) {
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(x, m[n][e]);
+                    x = fmaxf(x - Level<kTwo>::kBelow, m[n][e]);
                     keep[e] = m[n][e] == -INFINITY ? 0.0f : exp2_fast(m[n][e] - x);
                     m[n][e] = x;
                     l[n][e] *= keep[e];

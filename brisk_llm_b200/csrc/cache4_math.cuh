@@ -13,6 +13,16 @@ inline uint32_t multiprocessors() {
     return uint32_t(count);
 }
 
+// A weight is 2^(score - level) as one f16 or, for f32, two: what is below 2^-24 is lost, what is above 65504 does not fit. A level is set
+// kBelow under its row's maximum and stays until a score is 2^kMost above it, so that the largest weight of a row lies between 2^kBelow
+// and 2^kMost and the smallest that keep their bits lie as far below it as an f16 allows: 11 bits (one f16) down to 2^-21 of the
+// largest, 22 (two) down to 2^-15, to within 2^-32 and 2^-37 of the largest from there. With the level at the maximum those were 2^-25, and a
+// tail of 32 000 equal weights behind one heavy position 1e-4 off. The f32 level moves a little more often for it (past 2^3 times the
+// maximum it was set by instead of 2^8).
+template <bool TWO> struct Level {
+    static constexpr float kBelow = TWO ? 12.0f : 7.0f, kMost = 15.0f;
+};
+
 #ifdef __CUDACC__
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }

@@ -294,10 +294,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     __syncwarp();
                     if (kTwo && j % G::kFlush == 0) add_up(j > G::kFlush);
                 }
-                // the maximum moves only where a score is 2^8 above it: weights up to 256 fit f16 as well as those up to 1 do
-                const bool above = top > m + 8.0f;
+                // the level (see Level) moves only where a weight would no longer fit
+                const bool above = top > m + Level<kTwo>::kMost;
                 if (__any_sync(0xffffffffu, above)) {
-                    const float next = above ? top : m, keep = m == next ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - next);
+                    const float next = above ? top - Level<kTwo>::kBelow : m, keep = m == next ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(m - next);
                     m = next;
                     l *= keep;
                     if (kTwo && j >= G::kFlush) scale_columns(lanes + G::kTotal, keep);
