@@ -3,7 +3,8 @@
 //   k_scales, v_scales  [pages][kv_heads][page_size][dim / 32] f16
 // a position's row of a head being dim / 32 blocks of 32 values in the byte order of Q4_0: byte j holds value j in its low and value
 // j + 16 in its high four bits, a value is (n - 8) d. The scales that the append kernel writes have 8 significant bits, so that the
-// product - 3 bits and a sign times 8 - is an f16 number: kernels that multiply in f16 multiply the stored values themselves.
+// product - 3 bits and a sign times 8 - is an f16 number where the scale is below 8192: kernels that multiply in f16 multiply the stored
+// values themselves. For larger scales see past_f16 (cache4_math.cuh).
 #pragma once
 
 #include <mutex>

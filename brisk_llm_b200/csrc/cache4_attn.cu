@@ -358,8 +358,16 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                 }
             }
         }
+        // Values past what an f16 holds among those that the tile's rows see (see past_f16; the keys' scales are multiplied in 32 bits).
+        bool large;
+        {
+            const __half2* d = reinterpret_cast<const __half2*>(st + G::kVs + lane * G::kScales);  // of the lane's position
+            __half2 most = larger(d[0], d[D / 64 - 1]);
+            if (D == 256) most = larger(most, larger(d[1], d[2 % (D / 64)]));
+            large = past_f16(__hmax(__low2half(most), __high2half(most))) && (whole || (base + int(lane) >= lo && base + int(lane) <= hi));
+        }
         // The level (see Level) moves only where a weight would no longer fit.
-        bool above = false;
+        bool above = large;
         float top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -369,10 +377,19 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                 above = above || top[n][e] > m[n][e] + Level<kTwo>::kMost;
             }
         }
+        bool fold = false;
         if (__any_sync(0xffffffffu, above)) {
+            fold = __any_sync(0xffffffffu, large);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float keep[2];
+                if (fold) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        m[n][e] -= kFoldBits;
+                        l[n][e] *= kUnfold;
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     float x = top[n][e];
@@ -440,6 +457,10 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
             }
             pair[0] = __halves2half2(d[0], d[1]);
             pair[1] = __halves2half2(d[2], d[3]);
+            if (fold) {
+                pair[0] = __hmul2(pair[0], __float2half2_rn(kFold));
+                pair[1] = __hmul2(pair[1], __float2half2_rn(kFold));
+            }
         };
         if constexpr (kTwo) {
             // A product cuts its sum off at 24 bits: adding to a long sum each time loses a third of a bit of it per product, all one way. The tile's
@@ -493,6 +514,16 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
                             for (int n = 0; n < NT; ++n) mma16816(o[x * 4 + z * 2 + u][n], v0[2 * u], v0[2 * u + 1], v1[2 * u], v1[2 * u + 1], p_high[h][n][0], p_high[h][n][1]);
                         }
                     }
+                }
+            }
+        }
+        if (fold) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    m[n][e] += kFoldBits;
+                    l[n][e] *= kFold;
                 }
             }
         }

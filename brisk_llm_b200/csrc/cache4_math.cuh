@@ -39,9 +39,18 @@ __device__ __forceinline__ float exp2_fast(float x) {
 __device__ __forceinline__ uint32_t bits(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ __half2 halves(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 
+// From 8192 on -8 times a scale is past the largest f16, while scales are held up to 65280. The kernel of few rows folds a tile of positions
+// that holds such a scale of values: their scales are an eighth (65280 / 8 = 8160) and the weights 8 times what they are, for which the
+// level is 3 less, and the running sum 8 times as much, while the tile lasts; what Level says of the largest weight holds as it is. Eighths
+// are exact for scales from 2^-14 on; a value of a smaller one that shares its tile with one of 8192 is rounded to 2^-21. (Scales of
+// keys are multiplied in 32 bits there.) The kernel of many rows computes such rows in another way.
+constexpr float kFold = 0.125f, kUnfold = 8.0f, kFoldBits = 3.0f;
+__device__ __forceinline__ bool past_f16(__half scale) { return __hge(__habs(scale), __half(8192.0f)); }
+__device__ __forceinline__ __half2 larger(__half2 a, __half2 b) { return __hmax2(__habs2(a), __habs2(b)); }
+
 // The eight numbers of a word, n - 8 times the scale, as four pairs: (low of bytes 0, 2), (high of 0, 2), (low of 1, 3), (high of 1, 3).
 // A number set into the mantissa of 1024 (or, 16 times it, of 1024) is exact, so is n - 8, and so is the product with a scale of 8
-// bits: three instructions a pair and no rounding.
+// bits that is not past_f16: three instructions a pair and no rounding.
 __device__ __forceinline__ void widen(uint32_t w, __half2 scale, uint32_t (&v)[4]) {
     const uint32_t magic = 0x64006400u, u = w >> 8;
     const __half2 bias = halves(0x64086408u), sixteenth = halves(0x2c002c00u), less = halves(0xd480d480u);  // 1032, 1 / 16, -72

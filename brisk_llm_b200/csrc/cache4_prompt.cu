@@ -93,7 +93,64 @@ template <int N> __device__ __forceinline__ void fewer_registers() { asm volatil
 struct Bars {
     uint64_t q_full[2], k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], s_free, p_full[2], o_done[2], drained;
     uint32_t tmem;
+    uint32_t large;  // a scale was past_f16; of this CTA's, and behind the cluster's last barrier of its other CTAs' as well
 };
+
+// One row by a warp, in 32 bits from the cache as it lies, a lane to a position for the scores and to D / 32 values for the result.
+template <class T, int D>
+__device__ __forceinline__ void attend_row(const Cache4& c, const Cache4Batch& b, uint32_t sequence, uint32_t kv, const T* q, T* out, int first, int last, float scale) {
+    constexpr int kBlocks = D / 32, kBytes = D / 64;  // of a lane: kBytes of the row
+    const uint32_t lane = threadIdx.x & 31, block = lane * kBytes / 16, byte = lane * kBytes % 16;
+    float m = -INFINITY, l = 0.0f, o[2 * kBytes] = {};
+    for (long long base = first & ~31; base <= last; base += 32) {
+        const int p = int(base + lane);
+        const bool sees = base + lane <= last && p >= first;
+        const int32_t page = sees ? page_of(c, b, sequence, uint32_t(p) >> c.page_shift) : -1;
+        const size_t at = ((size_t(max(page, 0)) * c.kv_heads + kv) * c.page_size + (uint32_t(p) & (c.page_size - 1))) * kBlocks;
+        float score = 0.0f;
+        if (page >= 0) {
+#pragma unroll 1
+            for (int x = 0; x < 4 * kBlocks; ++x) {  // words
+                const uint32_t word = reinterpret_cast<const uint32_t*>(c.k_quants + at * 16)[x];
+                const T* y = q + x / 4 * 32 + x % 4 * 4;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum = fmaf(float(int(word >> (8 * i) & 15) - 8), to_float(y[i]), sum);
+                    sum = fmaf(float(int(word >> (8 * i + 4) & 15) - 8), to_float(y[i + 16]), sum);
+                }
+                score = fmaf(sum, __half2float(c.k_scales[at + x / 4]), score);
+            }
+        }
+        score = sees ? score * scale : -INFINITY;
+        const float next = fmaxf(m, warp_max(score)), less = next == -INFINITY ? 0.0f : next, keep = m == -INFINITY ? 0.0f : exp2_fast(m - less), w = exp2_fast(score - less);
+        m = next;
+        l = fmaf(l, keep, warp_sum(w));
+#pragma unroll
+        for (int i = 0; i < 2 * kBytes; ++i) o[i] *= keep;
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const float of = __shfl_sync(0xffffffffu, w, i);
+            const int32_t there = __shfl_sync(0xffffffffu, page, i);
+            const size_t place = __shfl_sync(0xffffffffu, (unsigned long long)at, i);
+            if (there >= 0) {
+                const float d = of * __half2float(c.v_scales[place + block]);
+                const uint8_t* n = c.v_quants + (place + block) * 16 + byte;
+#pragma unroll
+                for (int x = 0; x < kBytes; ++x) {
+                    o[2 * x] = fmaf(float(int(n[x] & 15) - 8), d, o[2 * x]);
+                    o[2 * x + 1] = fmaf(float(int(n[x] >> 4) - 8), d, o[2 * x + 1]);
+                }
+            }
+        }
+    }
+    const float inverse = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+#pragma unroll
+    for (int x = 0; x < kBytes; ++x) {
+        put(out + block * 32 + byte + x, o[2 * x] * inverse);
+        put(out + block * 32 + byte + x + 16, o[2 * x + 1] * inverse);
+    }
+}
 
 // softmax(q k) v for 256 rows (or 128) - tokens times the query heads of one key/value head - of one sequence, in two tiles of 128 rows that
 // take turns on the tensor cores. Four warpgroups: one for each tile's softmax, a thread to a row (its maximum and sum need no other); one
@@ -103,6 +160,10 @@ struct Bars {
 // The head's values lie in Q and K in the order in which a 4-bit word yields them. V is widened with neighbouring positions side by side, as
 // the product wants them: two words of two positions give pairs of one dim.
 // Where rows are few for the SMs, up to four CTAs of a cluster share a row's positions and join at the end.
+// The converters look at every scale. Where one was past_f16, which no model's keys and values are meant to be, the operand tiles hold infinities:
+// the CTA's rows are then computed again without them (attend_row), as exactly and far slower (one such value among 512 tokens of 32 heads:
+// 0.04 ms became 4.3). Folding such tiles would have to be agreed upon before each tile's keys are widened, which cost every call:
+// 4096 tokens 178 us became 195 to 220, where looking costs 3.
 // Every wait is bounded; one that runs out leaves NaN in the rows of its tile.
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a, uint32_t rows_per_cta) {
@@ -161,6 +222,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             }
             mbar_init(&bar->s_free, 4);
             mbar_init(&bar->drained, 1);
+            bar->large = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         __syncwarp();
@@ -346,8 +408,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) + __uint_as_float(y[i]));
             }
         };
+        const volatile uint32_t* large = &bar->large;
+        auto attend_rows = [&](uint32_t begin_at, uint32_t step) {
+            for (uint32_t x = begin_at; x < rows; x += step) {
+                const uint32_t of = (row0 + x) / group, h = kv * group + row0 + x - of * group;
+                attend_row<T, D>(c, b, sequence, kv, static_cast<const T*>(a.q) + size_t(first_row + of) * a.q_stride + size_t(h) * D,
+                                 static_cast<T*>(a.out) + size_t(first_row + of) * a.out_stride + size_t(h) * D, first_of(of), last_of(of), a.scale * 1.4426950408889634f);
+            }
+        };
         if (S == 1) {
-            if (works) {
+            if (works && !dead && *large != 0) {  // written before the values of the last tile were handed on
+                attend_rows(warp, 4 * halves_used);
+            } else if (works) {
                 const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
 #pragma unroll
                 for (int ch = 0; ch < D / 32; ++ch) {
@@ -396,8 +468,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     }
                 }
             }
+            if (tid == 0 && *large != 0) {
+                for (uint32_t k = 0; k < S; ++k) *cluster.map_shared_rank(&bar->large, k) = 1;
+            }
             cluster_meet();
-            if (real) {
+            if (*large != 0) {
+                attend_rows(warp * S + rank, 8 * S);
+            } else if (real) {
                 float most = -INFINITY, sum = 0.0f, by[kMostSplits];
                 for (uint32_t k = 0; k < S; ++k) most = fmaxf(most, sums[k * 256 + at].x);
 #pragma unroll
@@ -491,6 +568,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                 value_scale[i] = there ? c.v_scales[at + i * kBlocks + value_block] : __half(0.0f);
             }
         };
+        __half2 most = __half2half2(__half(0.0f));  // of the scales' magnitudes
         ask_pages(0);
         load_keys(0);
         load_values(0);
@@ -504,6 +582,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             for (int i = 0; i < kKeys; ++i) {
                 const uint32_t p = uint32_t(key_position(i)), w[4] = {key[i].x, key[i].y, key[i].z, key[i].w};
                 const __half2 d = __half2half2(key_scale[i]);
+                most = larger(most, d);
                 unsigned char* row = tile_k + (block >> 1) * (kN * 128) + p * 128;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
@@ -523,7 +602,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             if (has_values) {
                 __half2 d[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = __halves2half2(value_scale[2 * i], value_scale[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    d[i] = __halves2half2(value_scale[2 * i], value_scale[2 * i + 1]);
+                    most = larger(most, d[i]);
+                }
                 unsigned char* panel = tile_v + (group8 >> 3) * (D * 128);
 #pragma unroll
                 for (int x = 0; x < kWords; ++x) {
@@ -541,6 +623,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     }
                 }
             }
+            if (past_f16(__hmax(__low2half(most), __high2half(most)))) bar->large = 1;
             async_proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar->v_full[slot]);

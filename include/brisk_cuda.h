@@ -279,8 +279,9 @@ int brisk_cuda_argmax_static(const float* logits, uint32_t vocab, uint32_t rows,
  * A head's row of one position is head_dim / 32 blocks of 32 values: a scale d, and 16 bytes in the order of a Q4_0 block (byte j: value j
  * in the low, value j + 16 in the high four bits); a value is (n - 8) d. Appending chooses d = -m / 8, m the block's value of largest
  * magnitude (the positive one of two), rounded to 8 significant bits and kept as f16 (at most 65280), and n = floor(x / d + 8.5)
- * within 0 .. 15 (8 where d is 0). With 8 significant bits a value is an f16 number exactly. A NaN is stored as 0, an infinity as
- * the largest value of its block. */
+ * within 0 .. 15 (8 where d is 0). With 8 significant bits a value is an f16 number exactly, up to 65 280; past that (d of 8192 and more,
+ * values up to 522 240) it is none, and attention takes slower ways that give the same. A NaN is stored as 0, an infinity as the
+ * largest value of its block. */
 typedef struct brisk_cuda_cache4 {
     void* k_quants; /* [pages][kv_heads][page_size][head_dim / 2] bytes; every plane starts on a 16-byte boundary */
     void* k_scales; /* [pages][kv_heads][page_size][head_dim / 32] f16 */

@@ -1,12 +1,18 @@
-"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest. Against the definition, both kernels of the
-attention: few rows and many."""
+"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest, keys and values past what an f16 holds.
+Against the definition, both kernels of the attention: few rows and many."""
 import numpy as np
 import pytest
 
+import cache4_oracle as O
 import helpers as H  # noqa: F401  (puts the repository on sys.path)
-from test_gpu_cache4 import HALF_STEP, rounded
+from test_gpu_cache4 import HALF_STEP, World, rounded
 
 pytestmark = pytest.mark.gpu
+
+
+def torch_type(name):
+    from test_gpu_cache4 import torch_types
+    return torch_types()[name]
 
 
 @pytest.mark.parametrize("type,dim,sequences,tokens,context,nats", [
@@ -55,6 +61,78 @@ def test_heavy_positions_and_a_long_even_tail(type, dim, sequences, tokens, cont
     assert (err <= bound).all(), (err.max(), bound.min())
 
 
-def torch_type(name):
-    from test_gpu_cache4 import torch_types
-    return torch_types()[name]
+def bound(q, k, v, ref, type, scale, context):
+    """As test_gpu_cache4's tolerance(), but of each row by what that row sees - its own largest score and value - so that a position behind
+    it widens nothing. Scores: the products' magnitudes carry 2^-22 and their sum dim * 2^-24; a part of an f32 query is at least
+    2^-35 of the row's largest wide. A weight has 2^-22 (f32) or 2^-12 of itself, and is not known below 2^-37 (2^-32) of the largest."""
+    n, dim, group = k.shape[0], k.shape[2], q.shape[1] // k.shape[1]
+    out = np.empty_like(ref)
+    small, floor = (2.0 ** -22, 2.0 ** -37) if type == "f32" else (2.0 ** -12, 2.0 ** -32)
+    for h in range(q.shape[1]):
+        kh, vh = np.abs(k[:, h // group]), np.abs(v[:, h // group]).max(1)
+        size = np.abs(q[:, h]) @ kh.T * (2.0 ** -22 + dim * 2.0 ** -24) + np.abs(q[:, h]).max(1)[:, None] * 2.0 ** -35 * kh.sum(1)
+        for r in range(len(q)):
+            sees = context + r + 1
+            out[r, h] = vh[:sees].max() * (2 * scale * size[r, :sees].max() + 2 * small + (16 + n / 8) * 2.0 ** -24 + sees * floor)
+    return out + HALF_STEP[type] * np.abs(ref) + 1e-7
+
+
+def compare(got, q, k, v, type, context):
+    scale = q.shape[2] ** -0.5
+    ref = O.attention(q, k, v, context, scale)
+    err = np.abs(got - ref)
+    assert np.isfinite(got).all(), np.argwhere(~np.isfinite(got))[:4]
+    assert (err <= bound(q, k, v, ref, type, scale, context)).all(), err.max()
+    return err, ref
+
+
+LARGE = {"f32": [1e5, np.inf, -65504.0, 3e38, -np.inf], "bf16": [1e5, np.inf, -65504.0, 3e38, -np.inf], "f16": [65504.0, np.inf, -65504.0, 65408.0, -np.inf]}
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (128, 3), (256, 3), (64, 200), (128, 200), (256, 60), (128, 420)])
+def test_values_past_an_f16(dim, tokens, type):
+    """Values of up to 522 240 and infinities, appended among others: rows before them are as if they were not there, rows behind them are
+    what the stored values give."""
+    heads, kv, context = 8 if tokens < 100 else 32, 2, 400
+    n = context + tokens
+    w = World(31, kv, dim, [0], [n])
+    k, v = (w.rng.standard_normal((n, kv, dim)) for _ in range(2))
+    for i, x in enumerate(LARGE[type]):
+        v[n - tokens // 2 - 1 - 37 * (i % 2), i % kv, (11 * i) % dim] = x
+    v[130, 0, 3] = 1e-5  # a small one in a block of its own
+    v[130, 0, 4:32], v[130, 0, :3] = 0.0, 0.0
+    k, v = (rounded(x, type).to(w.device) for x in (k, v))
+    w.cache.append(w.batch, None, k, v)
+    kk, vv = (O.values(*O.quantise(x.float().cpu().numpy())) for x in (k, v))
+    from brisk_llm_b200 import cache4
+    batch = cache4.Batch(w.dev(np.array([context], np.int32)), tokens, page_table=w.batch.page_table, max_length=n)
+    q = rounded(w.rng.standard_normal((tokens, heads, dim)), type).to(w.device)
+    got = w.cache.attention(batch, q, out=q.new_empty(q.shape)).double().cpu().numpy()
+    ref = O.attention(q.double().cpu().numpy(), kk, vv, context, dim ** -0.5)
+    tops = {"f16": 65504.0}.get(type, np.inf)  # what an f16 result cannot hold is not asked for
+    here = np.abs(ref) < tops * 0.99
+    err = np.abs(got - ref)
+    assert here.mean() > 0.5 and np.isfinite(got[here]).all(), np.argwhere(~np.isfinite(got) & here)[:4]
+    assert (err <= bound(q.double().cpu().numpy(), kk, vv, ref, type, dim ** -0.5, context))[here].all()
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (128, 3), (256, 3), (64, 200), (128, 200), (256, 60), (128, 420)])
+def test_keys_past_an_f16(dim, tokens, type):
+    """Keys of up to 522 240 and infinities in dims that the queries have next to nothing in: their scores are of ordinary size."""
+    heads, kv, context = 8 if tokens < 100 else 32, 2, 400
+    n = context + tokens
+    w = World(32, kv, dim, [0], [n])
+    k, v = (w.rng.standard_normal((n, kv, dim)) for _ in range(2))
+    q = w.rng.standard_normal((tokens, heads, dim))
+    q[:, :, :32] *= 2e-5
+    for i, x in enumerate(LARGE[type]):
+        k[n - tokens // 2 - 1 - 37 * (i % 2), i % kv, 3 + 5 * i] = x
+    k, v, q = (rounded(x, type).to(w.device) for x in (k, v, q))
+    w.cache.append(w.batch, None, k, v)
+    kk, vv = (O.values(*O.quantise(x.float().cpu().numpy())) for x in (k, v))
+    from brisk_llm_b200 import cache4
+    batch = cache4.Batch(w.dev(np.array([context], np.int32)), tokens, page_table=w.batch.page_table, max_length=n)
+    got = w.cache.attention(batch, q).double().cpu().numpy()
+    compare(got, q.double().cpu().numpy(), kk, vv, type, context)
