@@ -9,7 +9,7 @@
 
 #include <mutex>
 
-#include "common.cuh"
+#include "kernels.h"
 
 namespace bk {
 
@@ -48,6 +48,7 @@ struct Cache4Attend {
     uint32_t heads = 0, window = 0;
     float scale = 0.0f;
     int wide = 0;
+    WaitBound bound;  // of the waits of the many-rows kernel; error may be null: only the NaN then says that one ran out
 };
 
 // What a kernel needs set once for each device (its opt-in to shared memory and cluster sizes), before its first launch there, whichever of

@@ -164,7 +164,7 @@ __device__ __forceinline__ void attend_row(const Cache4& c, const Cache4Batch& b
 // the CTA's rows are then computed again without them (attend_row), as exactly and far slower (one such value among 512 tokens of 32 heads:
 // 0.04 ms became 4.3). Folding such tiles would have to be agreed upon before each tile's keys are widened, which cost every call:
 // 4096 tokens 178 us became 195 to 220, where looking costs 3.
-// Every wait is bounded; one that runs out leaves NaN in the rows of its tile.
+// Every wait is bounded; one that runs out leaves NaN in the rows of its tile and sets the caller's error word, where there is one.
 template <class T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const Cache4 c, const Cache4Batch b, const Cache4Attend a, uint32_t rows_per_cta) {
     constexpr bool kTwo = sizeof(T) == 4;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
     const int all_tiles = hi >= lo ? (hi - (lo & ~(kN - 1))) / kN + 1 : 0, halves_used = rows > 128 ? 2 : 1;
     const int each = (all_tiles + int(S) - 1) / int(S), before = min(int(rank) * each, all_tiles), tiles = min(each, all_tiles - before);
     const int begin = (lo & ~(kN - 1)) + before * kN;
-    const long long limit = kTcWaitCycles;
+    const long long limit = a.bound.cycles;
     bool dead = bar->tmem != 0;
 
     if (warp < 8) {
@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
         ask_pages(1);
         for (int j = 0; j < tiles; ++j) {
             const uint32_t slot = j & 1;
+            if (uint32_t(j) == a.bound.withheld) dead = true;
             if (j >= 2) mbar_wait_warp(&bar->k_free[slot], (j >> 1) - 1 & 1, dead, limit);
             if (dead) break;
             unsigned char* tile_k = smem + G::kKAt + slot * G::kK;
@@ -703,6 +704,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
         cluster_meet();
         cluster_meet();
     }
+    if (dead && lane == 0 && a.bound.error != nullptr) atomicOr(a.bound.error, 1u);
     release_next();
     __syncwarp();
     tc_fence_before();

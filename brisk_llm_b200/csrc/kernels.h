@@ -65,14 +65,14 @@ constexpr uint32_t kPeerSlotPairs = 65536;
 void launch_tp_peer_exchange(uint2* const* bufs_dev, uint32_t* epoch, unsigned int* error, uint32_t tp, uint32_t rank, uint32_t slot_pairs,
                              const float* local, float* dst, uint32_t rows_l, bool add, cudaStream_t s);
 
-// ---- bounded waits of the kernels in tensor memory (gemm_k_tc.cu, and gemm_tc.cu: BRISK_CUDA_GEMM=tc) ----
+// ---- bounded waits of the kernels in tensor memory (gemm_k_tc.cu, cache4_prompt.cu, and gemm_tc.cu: BRISK_CUDA_GEMM=tc) ----
 constexpr long long kTcWaitCycles = 2000000000ll;  // about a second: a wait that lasts this long has failed
 // `error`, a word of the caller's in device memory, is non-zero after a launch with a wait that ran out. It belongs to one caller: read
 // and cleared by several, one would take the other's garbage for results.
 struct WaitBound {
     unsigned int* error = nullptr;
     long long cycles = kTcWaitCycles;
-    uint32_t withheld = 0xffffffffu;  // tests only: the step of a CTA's walk whose weights are never brought
+    uint32_t withheld = 0xffffffffu;  // tests only: the step of a CTA's walk whose weights, or keys and values, are never brought
 };
 // BRISK_CUDA_TEST_TC_TIMEOUT (tests only), for the bounds made while it is set. 1: the word is set from the start, as a wait that ran
 // out leaves it. 2 + k: the weights of step k are withheld, and the waits for them run out after 50 us. Every access stays in bounds and

@@ -225,7 +225,7 @@ struct Session {
     DevBuffer peer_buf, peer_table, peer_state;  // peer_state: [0] the next tag, [1] the error word
     std::vector<void*> peer_mapped;              // what cudaIpcOpenMemHandle returned (closed with the session)
     bool peer_on = false;
-    DevBuffer tc_error;  // set by a wait of this session's multiplies in tensor memory that ran out
+    DevBuffer tc_error;  // set by a wait of this session's kernels in tensor memory (multiplies, attention over 4 bits) that ran out
     WaitBound tc_bound;
     unsigned int* step_error_host = nullptr;  // pinned copy of the kernel's barrier-timeout word
     uint64_t persistent_steps = 0;
@@ -1045,6 +1045,7 @@ struct Session {
         Cache4Attend at;
         at.q = q_b.p; at.out = attended_b.p; at.q_stride = at.out_stride = q_dim_l;
         at.heads = heads_l; at.window = L.slides ? sliding_window : 0; at.scale = 1.0f / std::sqrt(static_cast<float>(head_dim));
+        at.bound = tc_bound;
         launch_cache4_attention(L.cache4, b, at, T_F32, true, stream);
         launches += 2;
     }
@@ -1103,7 +1104,7 @@ struct Session {
     // After the call's final synchronisation: did a wait of the persistent kernel run out? Asked after every call that ran it,
     // enqueued or replayed from a graph (step_on_device counts both).
     void queue_step_check() {
-        // The tcgen05 multiply has bounded waits: its error word, read with the results of a call that may have run it. (A word is
+        // The tcgen05 multiply, and the attention of many rows over a 4-bit cache, have bounded waits: their error word, read with the results of a call that may have run it. (A word is
         // a copy of its own, about 2 us at the end of every call.)
         if (batched) {
             BK_CUDA(cudaMemcpyAsync(step_error_host + 3, tc_error.p, sizeof(unsigned int), cudaMemcpyDeviceToHost, stream));
@@ -1116,7 +1117,7 @@ struct Session {
         if (step_error_host[3] != 0) {
             step_error_host[3] = 0;
             BK_CUDA(cudaMemsetAsync(tc_error.p, 0, sizeof(unsigned int), stream));
-            throw CudaError("cuda: a wait inside a multiply in tensor memory ran out; the results of this call are invalid");
+            throw CudaError("cuda: a wait inside a kernel in tensor memory ran out; the results of this call are invalid");
         }
         if (step_error_host[1] != 0) {
             step_error_host[1] = 0;
