@@ -245,7 +245,8 @@ __global__ void __launch_bounds__(32 * W, Split<D, NT, W, sizeof(T) == 4>::kResi
             }
         }
         if (lane == 0) {
-            row_scale[r] = fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 - up) << 23) * (kTwo ? 1.0f : 0x1p24f);
+            // (a query of 2^113 would take this past 32 bits: then scores are as large as they can be, and one position has the weight)
+            row_scale[r] = fminf(fabsf(a.scale) * 1.4426950408889634f * __uint_as_float(uint32_t(127 - up) << 23) * (kTwo ? 1.0f : 0x1p24f), 3e38f);
             row_last[r] = last_of(token);
             row_first[r] = first_of(token);
         }

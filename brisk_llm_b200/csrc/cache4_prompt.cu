@@ -366,7 +366,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
                     if (kTwo ? j % G::kFlush != 0 : j != 0) scale_columns(o_at, keep);
                 }
                 const float less = m == -INFINITY ? 0.0f : -m;
-                const f32x2 scale2 = pack2(scale, scale), less2 = pack2(less, less);
+                // A fused multiply and add takes the level, rounded, from the score that is not: past 2^20 that moves the weights, in the end past f16.
+                float by = scale;
+                if (__any_sync(0xffffffffu, fabsf(less) > 0x1p20f)) {
+#pragma unroll
+                    for (int i = 0; i < kN; ++i) x[i / 32][i % 32] = __float_as_uint(__uint_as_float(x[i / 32][i % 32]) * scale);
+                    by = 1.0f;
+                }
+                const f32x2 scale2 = pack2(by, by), less2 = pack2(less, less);
                 f32x2 sum[4] = {pack2(l, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
 #pragma unroll
                 for (int ch = 0; ch < kN / 32; ++ch) {

@@ -1,4 +1,4 @@
-"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest, keys and values past what an f16 holds.
+"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest, keys, values and queries past what an f16 holds.
 Against the definition, both kernels of the attention: few rows and many."""
 import numpy as np
 import pytest
@@ -136,3 +136,22 @@ def test_keys_past_an_f16(dim, tokens, type):
     batch = cache4.Batch(w.dev(np.array([context], np.int32)), tokens, page_table=w.batch.page_table, max_length=n)
     got = w.cache.attention(batch, q).double().cpu().numpy()
     compare(got, q.double().cpu().numpy(), kk, vv, type, context)
+
+
+@pytest.mark.parametrize("type", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,tokens", [(64, 1), (128, 3), (256, 3), (128, 200), (64, 200)])
+def test_queries_near_the_end_of_32_bits(dim, tokens, type):
+    """Scores of 10^35: one position of every row has all the weight."""
+    heads, kv, context = 4 if tokens < 100 else 32, 2, 300
+    n = context + tokens
+    w = World(33, kv, dim, [context], [tokens])
+    q = rounded(w.rng.standard_normal((tokens, heads, dim)) * 1e35, type).to(w.device)
+    got = w.cache.attention(w.batch, q).double().cpu().numpy()
+    k, v = w.values(0, n)
+    qs = q.double().cpu().numpy()
+    ref = O.attention(qs, k, v, context, dim ** -0.5)
+    for h in range(heads):  # no two scores of a row are within the rounding of one
+        s = np.sort(np.where(np.arange(n) <= context + np.arange(tokens)[:, None], qs[:, h] @ k[:, h * kv // heads].T, -np.inf), axis=1)
+        sure = s[:, -1] - s[:, -2] > dim * 2.0 ** -20 * np.abs(s).max(initial=0, where=np.isfinite(s))
+        assert sure.mean() > 0.9
+        assert (np.abs(got[:, h] - ref[:, h])[sure] <= HALF_STEP[type] * np.abs(ref[:, h])[sure] + 2.0 ** -11 * np.abs(v).max()).all()
