@@ -190,17 +190,30 @@ __device__ __forceinline__ void store_numbers(const Numbers& y, bool there, uint
     }
 }
 
-// x over its root mean square, times norm; a row is D / 8 lanes.
+// x over its root mean square, times norm; a row is D / 8 lanes. False: the row's squares leave the range of 32 bits, or so nearly that they
+// lose bits which the mean would show.
 template <class Real, int D>
-__device__ __forceinline__ void normed(Real (&x)[kLane], const float* norm, float eps) {
+__device__ __forceinline__ bool normed(Real (&x)[kLane], const float* norm, float eps) {
     Real sum = Real(0);
 #pragma unroll
     for (int j = 0; j < kLane; ++j) sum = fused(x[j], x[j], sum);
 #pragma unroll
     for (int o = D / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const Real scale = Real(1) / root(sum / Real(D) + Real(eps));
+    const Real mean = sum / Real(D) + Real(eps), scale = Real(1) / root(mean);
 #pragma unroll
     for (int j = 0; j < kLane; ++j) x[j] = x[j] * scale * Real(norm[j]);
+    return mean > Real(1e-27f) && mean < Real(1e38f);
+}
+
+// Queries' rows whose squares leave 32 bits, normed in 64.
+template <int D>
+__device__ __noinline__ void normed_wide(float* x, const float* norm, float eps) {
+    double wide[kLane];
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) wide[j] = double(x[j]);
+    normed<double, D>(wide, norm, eps);
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) x[j] = float(wide[j]);
 }
 
 // What a lane needs to turn its values of any row of the token: y = x c + other s, in pairs of values.
@@ -428,9 +441,20 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 12) cache4_append_kernel(co
 #pragma unroll
             for (int j = 0; j < kLane; ++j) x[j] = x[j] + bias[j];
         }
+        bool in_range = true;
         if (kKind != 2 && norm != nullptr) {
             norm += first;
-            normed<float, D>(x, norm, a.eps);
+            float before[kLane];
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) before[j] = x[j];
+            in_range = normed<float, D>(x, norm, a.eps);
+            if (kKind == 0 && __any_sync(0xffffffffu, !in_range)) {
+                normed_wide<D>(before, norm, a.eps);
+                if (!in_range) {
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j) x[j] = before[j];
+                }
+            }
         }
         if constexpr (kKind == 0) {
             if (a.rope_dim != 0) turned<false>(x, t, reinterpret_cast<float*>(pass[warp]));
@@ -447,11 +471,11 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 12) cache4_append_kernel(co
             const float within = most * reach;
             const size_t block = page_block + size_t(head) * c.page_size * (D / 32);
             Numbers numbers;
-            const bool sure = quick_numbers(x, within, numbers);
+            const bool sure = quick_numbers(x, within, numbers) && in_range;
             if (__any_sync(0xffffffffu, !sure)) {
                 bool doubt;
                 numbers = to_numbers<float>(x, within, &doubt);
-                if (__any_sync(0xffffffffu, doubt)) {
+                if (__any_sync(0xffffffffu, doubt || !in_range)) {
                     numbers = exact_numbers<T, D>(src, a.wide, bias, norm, a.eps, first, kKind == 1 ? a.rope_dim : 0, a.adjacent, turn, pass[warp]);
                 }
             }

@@ -1,11 +1,11 @@
-"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest, keys, values and queries past what an f16 holds.
-Against the definition, both kernels of the attention: few rows and many."""
+"""The 4-bit cache's operators at the ends of their range: weights far below a row's largest, keys, values and queries past what an f16 holds,
+rows whose squares leave 32 bits. Against the definition, both kernels of the attention: few rows and many."""
 import numpy as np
 import pytest
 
 import cache4_oracle as O
 import helpers as H  # noqa: F401  (puts the repository on sys.path)
-from test_gpu_cache4 import HALF_STEP, World, rounded
+from test_gpu_cache4 import HALF_STEP, World, rounded, same_scales
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +155,30 @@ def test_queries_near_the_end_of_32_bits(dim, tokens, type):
         sure = s[:, -1] - s[:, -2] > dim * 2.0 ** -20 * np.abs(s).max(initial=0, where=np.isfinite(s))
         assert sure.mean() > 0.9
         assert (np.abs(got[:, h] - ref[:, h])[sure] <= HALF_STEP[type] * np.abs(ref[:, h])[sure] + 2.0 ** -11 * np.abs(v).max()).all()
+
+
+@pytest.mark.parametrize("type,size", [("f32", 1e25), ("f32", 3e37), ("bf16", 1e30), ("f32", 1e-25), ("bf16", 1e-30), ("f16", 6e-8)])
+@pytest.mark.parametrize("dim,layout", [(64, "half"), (128, "adjacent"), (256, None)])
+def test_norms_of_rows_whose_squares_leave_32_bits(dim, layout, type, size):
+    import torch
+    from brisk_llm_b200 import cache4
+    w = World(34, 2, dim, [7], [9])
+    rng = w.rng
+    q, k, v = (rounded(rng.standard_normal((w.rows, h, dim)) * size, type).to(w.device) for h in (4, 2, 2))
+    q[3], k[3] = q[3] / size if size < 1e4 else q[3] * 0, k[3] * 0  # among rows of ordinary size and of zeros
+    qn, kn = (1 + 0.3 * rng.standard_normal(dim).astype(np.float32) for _ in range(2))
+    rotary = None if layout is None else cache4.Rotary(dim, 1e4, layout=layout)
+    turns = None if layout is None else 1e4 ** (-2.0 * np.arange(dim // 2) / dim) / (2 * np.pi)
+    got = w.cache.append(w.batch, q, k, v, rotary=rotary, q_norm=w.dev(qn), k_norm=w.dev(kn), eps=0.0)
+    position, at = w.positions(), None
+    with np.errstate(divide="ignore", invalid="ignore"):
+        wanted = [O.rotated(x.double().cpu().numpy(), position, norm=n, turns=turns, adjacent=layout == "adjacent") for x, n in ((q, qn), (k, kn))]
+    at = (w.table[0, position // w.page], slice(None), position % w.page)
+    kq, ks = O.quantise(wanted[1])
+    planes = w.planes()
+    assert same_scales(planes[1][at], ks) and np.array_equal(planes[0][at], kq)
+    here = ~np.isnan(wanted[0])
+    err = np.abs(got.double().cpu().numpy() - wanted[0])
+    top = np.abs(np.where(here, wanted[0], 0)).max(-1, keepdims=True)
+    assert (err <= HALF_STEP[type] * np.abs(wanted[0]) + 24 * 2.0 ** -24 * top + 1e-7)[here].all() and here.mean() > 0.8
+    assert not torch.isinf(got.float()).any()
