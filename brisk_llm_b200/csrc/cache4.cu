@@ -350,8 +350,9 @@ constexpr int kAppendWarps = 2;
 // A CTA of two warps to some of a token's rows, so that the token's angles are made once for them, in 64 bits: a far position turns a pair
 // thousands of times. A warp takes 32 / (D / 8) rows of q, of k or of v at a time. What is stored is what 64 bits give: a row is computed
 // in 32, with a bound on how far its values may be off, and once more in 64 where that bound reaches a border between two numbers or
-// two scales (a row in some hundreds). The bound, in half-ulps 2^-24 of the sum of a pair's magnitudes: bias 1, mean of squares
-// (8 + 5 + 1) / 2, root and quotient 2, two products 2, cos and sin and their sum 3: at most 15.
+// two scales (a row in some hundreds). The bound, in half-ulps 2^-24 of the sum of a pair's magnitudes: a value with its bias 1; the
+// mean of squares 2 of that, 8 + 5 of its sums and 1 of eps, halved by the root 8; root and quotient 2; products with both and the norm 2;
+// cos and sin, a product and a sum 3: 16 in the first order, 18 allowed.
 //
 // Rows are asked for first of all, so that they arrive while the angles are made; the loop then finds them in shared memory.
 template <class T, int D>
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(32 * kAppendWarps, 12) cache4_append_kernel(co
     const size_t page_block = ((size_t(max(page, 0)) * c.kv_heads) * c.page_size + slot) * (D / 32) + first / 32;
     __syncthreads();
     const Turns t = turns_of<D>(a.rope_dim, a.adjacent, cosine, sine);
-    const float reach = 0x1p-20f * fmaxf(1.0f, fabsf(a.attn_factor));
+    const float reach = 0x1.2p-20f * fmaxf(1.0f, fabsf(a.attn_factor));
     T* q_out = static_cast<T*>(a.q_out) + size_t(row) * a.q_out_stride + first;
     const uint32_t sub = lane / kLanes;
     // Rows of queries (kind 0), keys (1) or values (2): item `which` of its kind, the n-th that was asked for.
