@@ -665,8 +665,11 @@ extern "C" int brisk_cuda_rope_turns(uint32_t rope_dim, double base, double scal
         require(turns != nullptr && rope_dim != 0 && rope_dim % 2 == 0, "needs an even rotated width and an output for its turns");
         require(base > 0.0 && std::isfinite(base) && std::isfinite(scale), "needs a positive, finite rotation base and a finite scale");
         for (uint32_t i = 0; i < rope_dim / 2; ++i) {
+            require(factors == nullptr || (factors[i] != 0.0f && std::isfinite(factors[i])), "needs divisors of the angles that are finite and not 0");
             const double angle = scale * std::pow(base, -2.0 * double(i) / double(rope_dim));
-            turns[i] = (factors != nullptr ? angle / double(factors[i]) : angle) / 6.283185307179586476925286766559;
+            const double turn = (factors != nullptr ? angle / double(factors[i]) : angle) / 6.283185307179586476925286766559;
+            require(std::isfinite(turn), "needs a rotation whose angles are finite");
+            turns[i] = turn;
         }
     });
 }

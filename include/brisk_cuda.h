@@ -333,7 +333,7 @@ typedef struct brisk_cuda_cache4_rows {
     int32_t type; /* of q, k, v and q_out: BRISK_TYPE_F32, _F16 or _BF16 */
 } brisk_cuda_cache4_rows;
 
-/* turns[i] = scale * base^(-2 i / rope_dim) / factors[i] / 2 pi for i < rope_dim / 2 (factors may be NULL), HOST pointers: what a program
+/* turns[i] = scale * base^(-2 i / rope_dim) / factors[i] / 2 pi for i < rope_dim / 2 (factors, finite and not 0, may be NULL), HOST pointers: what a program
  * uploads once. Angles are made of them in 64 bits, so far positions rotate as exactly as near ones. */
 int brisk_cuda_rope_turns(uint32_t rope_dim, double base, double scale, const float* factors, double* turns, char* err, size_t errlen);
 
