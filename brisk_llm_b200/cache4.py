@@ -13,6 +13,7 @@ read on the device when the work runs: a captured call that is replayed sees wha
 from __future__ import annotations
 
 import ctypes as C
+import math
 import threading
 
 import torch
@@ -42,6 +43,8 @@ class Rotary:
         if self.width > head_dim or self.width % 2:
             _fail("the rotated width must be even and at most the head size")
         self.adjacent, self.attn_factor = int(layout == "adjacent"), float(attn_factor)
+        if self.attn_factor == 0.0 or not math.isfinite(self.attn_factor):
+            _fail("a rotation's factor on cos and sin must be finite and not 0")
         divisors = None
         if factors is not None:
             factors = torch.as_tensor(factors, dtype=torch.float32).cpu().contiguous()

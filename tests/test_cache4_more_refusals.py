@@ -29,3 +29,11 @@ def test_divisors_without_an_angle_are_refused(wrong):
 def test_angles_past_64_bits_are_refused():
     rc, text, _ = turns(base=1e-300, scale=1e200)
     assert rc != 0 and "angles are finite" in text
+
+
+@pytest.mark.parametrize("factor", [0.0, float("nan"), float("inf")])
+def test_a_rotary_s_factor_is_what_is_multiplied_by(factor):
+    from brisk_llm_b200 import cache4
+    with pytest.raises(RuntimeError, match="^cuda: .*factor"):
+        cache4.Rotary(64, 1e4, attn_factor=factor, device="cpu")
+    assert cache4.Rotary(64, 1e4, attn_factor=0.5, device="cpu").attn_factor == 0.5
