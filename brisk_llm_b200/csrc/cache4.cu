@@ -640,6 +640,16 @@ void check_device(const Cache4& c) {
     require(where.device == device, "is on another device than the current one");
 }
 
+// Whether no token's row of a touches a row of b: rows of `width` bytes, `stride` bytes apart. Rows of one stride may lie between one another, as
+// the parts of a fused buffer do.
+bool apart(const void* a, uint64_t a_stride, uint64_t a_width, const void* b, uint64_t b_stride, uint64_t b_width, uint64_t tokens) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    if (x + (tokens - 1) * a_stride + a_width <= y || y + (tokens - 1) * b_stride + b_width <= x) return true;
+    if (a_stride != b_stride) return false;
+    const uint64_t behind = (y >= x ? y - x : a_stride - (x - y) % a_stride) % a_stride;  // of b's rows behind a's, within a stride
+    return behind >= a_width && behind + b_width <= a_stride;
+}
+
 void check_type(int type) { require(type == T_F32 || type == T_F16 || type == T_BF16, "takes activations in f32, f16 and bf16"); }
 
 template <class Fn>
@@ -696,6 +706,13 @@ extern "C" int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const br
         require(rows->rope_dim == 0 || rows->rope_turns != nullptr, "needs the turns of the pairs it rotates");
         require(rows->eps >= 0.0f && std::isfinite(rows->eps), "needs a finite epsilon of at least 0");
         require(std::isfinite(rows->rope_attn_factor), "needs a finite factor on cos and sin");
+        if (rows->heads != 0) {
+            const uint64_t wide = uint64_t(rows->heads) * c.dim * size, narrow = kv * size, to = rows->q_out_stride * size;
+            require((rows->q == rows->q_out && rows->q_stride == rows->q_out_stride) || bk::apart(rows->q, rows->q_stride * size, wide, rows->q_out, to, wide, b.tokens),
+                    "writes its queries over q itself or apart from it");
+            require(bk::apart(rows->k, rows->k_stride * size, narrow, rows->q_out, to, wide, b.tokens) && bk::apart(rows->v, rows->v_stride * size, narrow, rows->q_out, to, wide, b.tokens),
+                    "cannot write its queries over keys and values");
+        }
         bk::Cache4Append a;
         a.q = rows->q; a.k = rows->k; a.v = rows->v; a.q_out = rows->q_out;
         a.q_stride = rows->q_stride; a.k_stride = rows->k_stride; a.v_stride = rows->v_stride; a.q_out_stride = rows->q_out_stride;
@@ -718,6 +735,7 @@ extern "C" int brisk_cuda_cache4_read(const brisk_cuda_cache4* cache, const bris
         require(k != nullptr && v != nullptr && bk::aligned(k, size) && bk::aligned(v, size), "needs outputs for keys and values on boundaries of their type");
         const uint64_t kv = uint64_t(c.kv_heads) * c.dim;
         require(k_stride >= kv && v_stride >= kv, "needs token strides of at least a token's heads (k, v)");
+        require(bk::apart(k, k_stride * size, kv * size, v, v_stride * size, kv * size, b.tokens), "cannot write its keys over its values");
         bk::check_device(c);
         bk::launch_cache4_read(c, b, k, v, k_stride, v_stride, type, static_cast<cudaStream_t>(stream));
     });
@@ -737,6 +755,8 @@ extern "C" int brisk_cuda_cache4_attention(const brisk_cuda_cache4* cache, const
         require(q != nullptr && out != nullptr && bk::aligned(q, size) && bk::aligned(out, size), "needs queries, and where the result goes, on boundaries of their type");
         require(q != out, "cannot write its result over the queries");
         require(q_stride >= uint64_t(heads) * c.dim && out_stride >= uint64_t(heads) * c.dim, "needs token strides of at least a token's heads (q, out)");
+        const uint64_t wide = uint64_t(heads) * c.dim * size;
+        require(bk::apart(q, q_stride * size, wide, out, out_stride * size, wide, b.tokens), "cannot write its result over the queries");
         bk::Cache4Attend a;
         a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.heads = heads; a.window = window;
         a.scale = scale != 0.0f ? scale : 1.0f / std::sqrt(float(c.dim));

@@ -312,7 +312,7 @@ typedef struct brisk_cuda_cache4_batch {
 } brisk_cuda_cache4_batch;
 
 /* One layer's projections of a batch: element (row, head, i) of q is at q[row * q_stride + head * head_dim + i], the others likewise
- * (strides in values; q, k and v may lie in one fused buffer, and q_out may be q). */
+ * (strides in values; q, k and v may lie in one fused buffer, and q_out may be q, with its stride; else it overlaps none of them). */
 typedef struct brisk_cuda_cache4_rows {
     const void* q; /* heads may be 0: keys and values only */
     const void* k;
@@ -343,7 +343,7 @@ int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const brisk_cuda_ca
 
 /* out[row][head] = sum over the positions j the row sees of softmax(scale * q . k_j) v_j: those up to its own, with a window only the last
  * `window` of them (0: all). Query head h reads key/value head h / (heads / kv_heads). scale 0: 1 / sqrt(head_dim). A row that sees
- * nothing is zeros. out may not be q. Sums and softmax statistics are held in 32 bits. Before they meet the values, weights are rounded to 22
+ * nothing is zeros. out may not overlap q. Sums and softmax statistics are held in 32 bits. Before they meet the values, weights are rounded to 22
  * bits with f32 queries and to 11 (f16) with the others; weights of less than 2^-15 (2^-21) of a row's largest to within 2^-37
  * (2^-32) of it. The kernel of many rows waits inside itself, for a second at most: a wait that runs out, which a sound device does not
  * know, leaves NaN in rows of out (a session's call returns an error instead). */
