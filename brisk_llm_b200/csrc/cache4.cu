@@ -623,6 +623,7 @@ Cache4Batch checked(const brisk_cuda_cache4_batch* in, const Cache4& c) {
     require(in->context != nullptr, "needs the positions before the batch (context)");
     require(in->query_start != nullptr || in->tokens % in->sequences == 0, "needs query_start where the tokens do not split evenly over the sequences");
     require(in->table_columns != 0 && uint64_t(in->table_columns) * c.page_size <= 0x7fffffffull, "needs 1 to 2^31 - 1 positions in a sequence's columns");
+    require(aligned(in->context, 4) && aligned(in->page_table, 4) && aligned(in->query_start, 4), "needs context, page_table and query_start on 4-byte boundaries");
     b.context = in->context; b.page_table = in->page_table; b.query_start = in->query_start;
     b.max_tokens = in->query_start == nullptr ? b.tokens / b.sequences : in->max_tokens != 0 && in->max_tokens < b.tokens ? in->max_tokens : b.tokens;
     const uint32_t most = b.columns * c.page_size;
@@ -704,6 +705,9 @@ extern "C" int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const br
         require((rows->k_stride >= kv && rows->v_stride >= kv), "needs token strides of at least a token's heads (k, v)");
         require(rows->rope_dim <= c.dim && rows->rope_dim % 2 == 0, "rotates an even width of at most the head size");
         require(rows->rope_dim == 0 || rows->rope_turns != nullptr, "needs the turns of the pairs it rotates");
+        require(bk::aligned(rows->rope_turns, 8), "needs the turns of the pairs on an 8-byte boundary");
+        require(bk::aligned(rows->q_norm, 4) && bk::aligned(rows->k_norm, 4) && bk::aligned(rows->q_bias, 4) && bk::aligned(rows->k_bias, 4) && bk::aligned(rows->v_bias, 4),
+                "needs norms and biases on 4-byte boundaries");
         require(rows->eps >= 0.0f && std::isfinite(rows->eps), "needs a finite epsilon of at least 0");
         require(std::isfinite(rows->rope_attn_factor), "needs a finite factor on cos and sin");
         if (rows->heads != 0) {

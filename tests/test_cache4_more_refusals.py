@@ -1,4 +1,5 @@
-"""More of what the calls of the 4-bit cache refuse: rotations without finite angles, outputs that overlap what is still to be read."""
+"""More of what the calls of the 4-bit cache refuse: rotations without finite angles, outputs that overlap what is still to be
+read, pointers off their boundaries."""
 import ctypes as C
 
 import numpy as np
@@ -81,3 +82,18 @@ def test_queries_over_keys_or_values_are_refused(kw, over):
 def test_keys_read_over_values_are_refused(v, k_stride, v_stride, over):
     call = read(cache(), batch(), v=v, k_stride=k_stride, v_stride=v_stride)
     assert refused(call, "over its values") == over, call
+
+
+@pytest.mark.parametrize("name", ["context", "page_table", "query_start"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_a_batch_off_its_boundaries_is_refused(name, off):
+    """Read as they are, these would end the process's context with a misaligned address."""
+    for call in (append(cache(), batch(**{name: P + off}), rows()), attention(cache(), batch(**{name: P + off})), read(cache(), batch(**{name: P + off}))):
+        assert refused(call, "4-byte boundaries"), call
+
+
+@pytest.mark.parametrize("name,off,message", [("rope_turns", 4, "8-byte"), ("rope_turns", 1, "8-byte")] +
+                         [(n, o, "norms and biases") for n in ("q_norm", "k_norm", "q_bias", "k_bias", "v_bias") for o in (1, 2, 3)])
+def test_rows_off_their_boundaries_are_refused(name, off, message):
+    call = append(cache(), batch(), rows(k=FAR, v=FAR, **{name: P + off}))
+    assert refused(call, message), call
