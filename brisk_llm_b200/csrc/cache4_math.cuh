@@ -19,6 +19,11 @@ inline uint32_t multiprocessors() {
 // largest, 22 (two) down to 2^-15, to within 2^-32 and 2^-37 of the largest from there. With the level at the maximum those were 2^-25, and a
 // tail of 32 000 equal weights behind one heavy position 1e-4 off. The f32 level moves a little more often for it (past 2^3 times the
 // maximum it was set by instead of 2^8).
+//
+// One f16, 11 bits, for f16 and bf16 queries: as many as the result has, or more; another part would double the products with the values. Against
+// 64 bits the results are 2.9e-4 off with f16 queries, 2.1e-4 with weights of 32 bits, and with bf16 ones 1.7e-3 either way: what is left is the
+// rounding of the result. Two, 22 bits, for f32: three would add half to the products again, and the errors are those of sums in 32 bits
+// without it (3e-7 to 8e-7; everything in 32 bits: 5e-7 to 1.2e-6).
 template <bool TWO> struct Level {
     static constexpr float kBelow = TWO ? 12.0f : 7.0f, kMost = 15.0f;
 };

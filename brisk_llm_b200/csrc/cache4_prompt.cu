@@ -156,7 +156,9 @@ __device__ __forceinline__ void attend_row(const Cache4& c, const Cache4Batch& b
 // take turns on the tensor cores. Four warpgroups: one for each tile's softmax, a thread to a row (its maximum and sum need no other); one
 // widens the 4-bit keys and values of 128 positions (64 where queries are two f16 parts) into the operand tiles of the products,
 // once for both tiles of rows; a warp of the last issues the products,
-//     S = Q K^T (both operands in shared memory),     O += P V (P in tensor memory, where the softmax wrote it over S).
+//     S = Q K^T (both operands in shared memory),     O += P V (P in tensor memory).
+// S is in columns 0 .. 127 for both tiles of rows: a softmax takes it into registers at once and gives it back by s_free, before it writes
+// a weight. The weights of tile i are in columns kW + 64 i, written between o_done (of the last) and p_full.
 // The head's values lie in Q and K in the order in which a 4-bit word yields them. V is widened with neighbouring positions side by side, as
 // the product wants them: two words of two positions give pairs of one dim.
 // Where rows are few for the SMs, up to four CTAs of a cluster share a row's positions and join at the end.

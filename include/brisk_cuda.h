@@ -270,11 +270,11 @@ int brisk_cuda_argmax_static(const float* logits, uint32_t vocab, uint32_t rows,
  * No counterpart in the reference (its cache is f16, contiguous, of one sequence). For embedders that keep the keys and values of
  * several sequences, or of long ones, in 28 % of the f16 bytes: rows are appended, attended to and read back by the three calls below.
  * Sessions created with BRISK_CUDA_FLAG_CACHE_4BIT run their layers over them. All pointers are DEVICE pointers on the current device unless
- * they are said to be host ones; `stream` is a cudaStream_t (NULL: the default stream). The calls launch on the stream and return: no
- * allocation, no synchronisation, no workspace, nothing kept. Pointers stand on boundaries of what they point to. So calls may overlap on several streams and from several threads as long as
- * none writes what another reads, and they may be captured into a graph and replayed, with context, page_table and query_start read at
- * every replay (make one call of the kind before the capture: the driver loads kernels when they are first used). They return 0, or -1
- * and a message in err before anything is launched.
+ * they are said to be host ones, on a boundary of what they point to; `stream` is a cudaStream_t (NULL: the default stream). The calls
+ * launch on the stream and return: no allocation, no synchronisation, no workspace, nothing kept. So calls may overlap on several streams
+ * and from several threads as long as none writes what another reads, and they may be captured into a graph and replayed, with context,
+ * page_table and query_start read at every replay (make one call of the kind before the capture: the driver loads kernels when they are
+ * first used). They return 0, or -1 and a message in err before anything is launched.
  *
  * A head's row of one position is head_dim / 32 blocks of 32 values: a scale d, and 16 bytes in the order of a Q4_0 block (byte j: value j
  * in the low, value j + 16 in the high four bits); a value is (n - 8) d. Appending chooses d = -m / 8, m the block's value of largest
