@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             }
             mbar_wait_warp(&bar->o_done[half], (tiles - 1) & 1, dead, limit);
             tc_fence_after();
+            mbar_wait_warp(&bar->v_full[(tiles - 1) & 1], (tiles - 1) >> 1 & 1, dead, limit);  // long complete: what the converters wrote before it is seen
         }
         // 32 values of the row's result, before they are divided by the sum of its weights
         auto result_of = [&](int ch, uint32_t (&x)[32]) {
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) cache4_prompt_kernel(const 
             }
         };
         if (S == 1) {
-            if (works && !dead && *large != 0) {  // written before the values of the last tile were handed on
+            if (works && !dead && *large != 0) {
                 attend_rows(warp, 4 * halves_used);
             } else if (works) {
                 const float inverse = dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);

@@ -63,3 +63,11 @@ def test_the_waits_of_the_many_rows_kernel_are_a_warp_s():
     assert not re.search(r"\bmbar_wait\(", text) and len(re.findall(r"\bmbar_wait_warp\(", text)) >= 6
     helper = open(os.path.join(CSRC, "tc.cuh")).read().split("void mbar_wait_warp(")[1].split("\n}")[0]
     assert helper.index("mbar_wait(") < helper.index("__any_sync") < helper.index("__syncwarp();")
+
+
+def test_what_the_converters_saw_is_read_behind_their_own_barrier():
+    """The softmax's warps ask whether a scale was past_f16 behind a wait for the last values, on which the converters arrive after they wrote it."""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, "cache4_prompt.cu")).read())
+    write, arrive = text.index("bar->large = 1"), text.index("mbar_arrive(&bar->v_full[slot])")
+    wait, read = text.index("mbar_wait_warp(&bar->v_full[(tiles - 1) & 1]"), text.index("*large != 0")
+    assert write < arrive and wait < read

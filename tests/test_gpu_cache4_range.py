@@ -182,3 +182,34 @@ def test_norms_of_rows_whose_squares_leave_32_bits(dim, layout, type, size):
     top = np.abs(np.where(here, wanted[0], 0)).max(-1, keepdims=True)
     assert (err <= HALF_STEP[type] * np.abs(wanted[0]) + 24 * 2.0 ** -24 * top + 1e-7)[here].all() and here.mean() > 0.8
     assert not torch.isinf(got.float()).any()
+
+
+@pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("window,scale", [(0, 0.0), (90, 0.0), (0, -0.05)])
+def test_large_values_and_keys_where_no_cluster_shares_a_row(window, scale, dim, type):
+    """CTAs enough for all SMs: each computes its rows alone, those that met a large scale twice. Two ragged sequences, one without any large
+    one; a window that leaves them behind; a scale below zero."""
+    from brisk_llm_b200 import cache4
+    heads, kv, context, tokens = 32, 8, [100, 31], [300, 120]
+    w = World(35, kv, dim, [0, 0], [c + t for c, t in zip(context, tokens)])
+    k, v = (w.rng.standard_normal((w.rows, kv, dim)) for _ in range(2))
+    q = w.rng.standard_normal((sum(tokens), heads, dim))
+    q[:, :, :32] *= 2e-5
+    for i, x in enumerate(LARGE[type]):
+        v[150 + i, 3, 7 * i] = x
+        k[170 + 11 * i, i + 1, 5 * i] = x
+    k, v, q = (rounded(x, type).to(w.device) for x in (k, v, q))
+    w.cache.append(w.batch, None, k, v)
+    batch = cache4.Batch(w.dev(np.array(context, np.int32)), sum(tokens), page_table=w.batch.page_table,
+                         query_start=w.dev(np.array([0, tokens[0], sum(tokens)], np.int32)), max_tokens=max(tokens), max_length=400)
+    got = w.cache.attention(batch, q, scale=scale, window=window).double().cpu().numpy()
+    kk, vv = (O.values(*O.quantise(x.float().cpu().numpy())) for x in (k, v))
+    qs, real = q.double().cpu().numpy(), scale or dim ** -0.5
+    for s in range(2):
+        rows, at = slice(sum(tokens[:s]), sum(tokens[:s + 1])), slice(int(w.start[s]), int(w.start[s + 1]))
+        ref = O.attention(qs[rows], kk[at], vv[at], context[s], real, window)
+        here = np.abs(ref) < (65504.0 * 0.99 if type == "f16" else np.inf)
+        err = np.abs(got[rows] - ref)
+        assert here.mean() > 0.9 and np.isfinite(got[rows][here]).all()
+        assert (err <= bound(qs[rows], kk[at], vv[at], ref, type, abs(real), context[s]))[here].all(), s
