@@ -780,9 +780,13 @@ void prompt_typed(const Cache4& c, const Cache4Batch& b, const Cache4Attend& in,
 // The kernel of few rows takes 16 at a time and spreads their positions over all SMs; a CTA of this one takes up to 256 rows and its positions one
 // after another. So this one needs rows enough, and the line is where the times of the two meet, in ns with bf16 heads of 128 (the other types and
 // heads move both alike): 30 and 1 for 17 positions of every 16 rows there, 10000 and 16 for a position of each round of CTAs here. us of few / many
-// rows: 64 times 32 rows after 2000 positions 21.2 / 21.0, after 8000 63 / 44, 128 times 32 after 4000 66 / 31, 256 times 32 at the start of a
-// prompt 23 / 12, 32 sequences of 36 rows after 3000 140 / 120, 8 of 18 after 2000 25 / 29; f32 27 / 25, 86 / 54, 89 / 38, 25 / 16, 183 / 157, 32 / 34.
-// With 32 rows or fewer most of a tile is empty: 32 sequences of 18 rows after 3000 96 / 121, f32 124 / 155.
+// rows, heads of 128 in bf16, f32, heads of 64 in bf16, f32:
+//     64 times 32 rows after 2000 positions    20.6 / 20.2   26.7 / 24.9   14.8 / 15.3   18.2 / 19.2
+//     the same after 8000                      60 / 41       82 / 57       42 / 32       54 / 46
+//     128 times 32 after 4000                  65 / 30       88 / 38       37 / 22       49 / 30
+//     256 times 32 at the start of a prompt    23 / 12       25 / 17       12.3 / 10.0   12.8 / 11.8
+//     32 sequences of 36 rows after 3000       139 / 114     179 / 165     90 / 84       111 / 126
+// With 32 rows or fewer most of a tile is empty: 32 sequences of 18 rows after 3000 96 / 121, f32 124 / 155. Heads of 256 have no form here.
 bool cache4_prompt_takes(const Cache4& c, const Cache4Batch& b, const Cache4Attend& a, int type) {
     const uint64_t rows = uint64_t(b.max_tokens) * (a.heads / c.kv_heads);
     if (c.dim > 128 || rows <= 32) return false;

@@ -343,10 +343,11 @@ int brisk_cuda_cache4_append(const brisk_cuda_cache4* cache, const brisk_cuda_ca
 
 /* out[row][head] = sum over the positions j the row sees of softmax(scale * q . k_j) v_j: those up to its own, with a window only the last
  * `window` of them (0: all). Query head h reads key/value head h / (heads / kv_heads). scale 0: 1 / sqrt(head_dim). A row that sees
- * nothing is zeros. out may not overlap q. Sums and softmax statistics are held in 32 bits. Before they meet the values, weights are rounded to 22
- * bits with f32 queries and to 11 (f16) with the others; weights of less than 2^-15 (2^-21) of a row's largest to within 2^-37
- * (2^-32) of it. The kernel of many rows waits inside itself, for a second at most: a wait that runs out, which a sound device does not
- * know, leaves NaN in rows of out (a session's call returns an error instead). */
+ * nothing is zeros. out may not overlap q. Sums and softmax statistics are held in 32 bits (a score of f16 or bf16 queries may lose two of
+ * them); scores past 32 bits leave NaN. Before they meet the values, weights are rounded to 22 bits with f32 queries and to 11 (f16) with
+ * the others; weights of less than 2^-15 (2^-21) of a row's largest to within 2^-37 (2^-32) of it. The kernel of many rows waits inside
+ * itself, for a second at most: a wait that runs out, which a sound device does not know, leaves NaN in rows of out (a session's call
+ * returns an error instead). */
 int brisk_cuda_cache4_attention(const brisk_cuda_cache4* cache, const brisk_cuda_cache4_batch* batch, int32_t type, const void* q, void* out, uint64_t q_stride,
                                 uint64_t out_stride, uint32_t heads, float scale, uint32_t window, void* stream, char* err, size_t errlen);
 
